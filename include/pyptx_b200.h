@@ -156,6 +156,51 @@ extern "C" {
  *   clears the fp32 dQ accumulator it keeps there with a stream-ordered memset.                      */
 #define PB200_K_FLASH_ATTN_BWD 16
 
+/* Mixture-of-experts token movement around the grouped GEMMs above: what makes their sorted rows and
+ * expert offsets, and what brings the rows back.  The reference takes pre-stacked rows
+ * (examples/blackwell/grouped_gemm.py:295-306) and has no counterpart.  T tokens with top_k choices
+ * each, entry i = t * top_k + j; R rows; H columns; PB200_F_OUT_BF16 = rows and tokens are bf16 (else f32).
+ *   PB200_K_MOE_ROUTE         dims = {T, top_k, E, block, R}   flags: PB200_F_IDS_S64
+ *       buffers: ids[T,top_k] s32 (s64) -> row_of[T,top_k], entry_of[R], offsets[E+1] s32
+ *       Entries sorted by expert, equal experts in entry order, each expert's rows padded to a multiple
+ *       of block.  Entries whose id lies outside [0, E), or whose row would be R or above, get row -1;
+ *       rows without an entry get entry -1; offsets are clipped to R.
+ *   PB200_K_MOE_DISPATCH      dims = {T, top_k, R, H}
+ *       buffers: x[T,H], row_of, entry_of -> rows[R,H] (zeros where entry_of < 0)
+ *   PB200_K_MOE_DISPATCH_FP8  dims = {T, top_k, R, H}          flags: PB200_F_IN_BF16
+ *       buffers: x[T,H] f32 (bf16), row_of, entry_of -> q[R,H] e4m3, scale[R,ceil(H/128)] f32
+ *   PB200_K_MOE_DISPATCH_BWD  dims = {T, top_k, R, H}
+ *       buffers: row_of, d_rows[R,H] -> dx[T,H]
+ *   PB200_K_MOE_COMBINE       dims = {T, top_k, R, H}
+ *       buffers: rows[R,H], weights[T,top_k] f32, row_of -> out[T,H] = sum over j of weights * rows
+ *   PB200_K_MOE_COMBINE_BWD   dims = {T, top_k, R, H}
+ *       buffers: rows, weights, row_of, entry_of, dout[T,H] -> d_rows[R,H], d_weights[T,top_k] f32
+ * Rows outside [0, R) in row_of count as dropped.  Sums are f32 in the order of j, without atomics.   */
+#define PB200_K_MOE_ROUTE        17
+#define PB200_K_MOE_DISPATCH     18
+#define PB200_K_MOE_DISPATCH_FP8 19
+#define PB200_K_MOE_DISPATCH_BWD 20
+#define PB200_K_MOE_COMBINE      21
+#define PB200_K_MOE_COMBINE_BWD  22
+/* Quantisation to e4m3 with an f32 scale for each 1 x 128 (activations) or 128 x 128 (weights) block:
+ * s = max(amax / 448, 2^-120), q = e4m3(x * (1 / s)), every step f32 and rounded to nearest.
+ *   dims = {M, K, block_rows (1 | 128)}   flags: PB200_F_IN_BF16
+ *   buffers: x[M,K] f32 (bf16) -> q[M,K] e4m3, scale[ceil(M/block_rows),ceil(K/128)] f32                */
+#define PB200_K_FP8_QUANTIZE     23
+/* GEMM of such operands: D[m,n] = sum over 128-wide blocks b of K of
+ *   a_scale[m,b] * b_scale[n/128,b] * sum_{k in b} A[m,k] B_T[n,k]
+ * (the 8-bit counterpart of PB200_K_GEMM_1SM and PB200_K_GROUPED_GEMM_VARLEN; the reference has no
+ * 8-bit GEMM).  K % 16 == 0, N % 8 == 0, M free.   flags: PB200_F_OUT_BF16
+ *   PB200_K_FP8_GEMM          dims = {M, N, K}
+ *       buffers: A[M,K] e4m3, a_scale[M,ceil(K/128)] f32, B_T[N,K] e4m3,
+ *                b_scale[ceil(N/128),ceil(K/128)] f32 -> D[M,N] f32 (or bf16)
+ *   PB200_K_FP8_GROUPED_GEMM  dims = {G, M_total, N, K}
+ *       buffers: A[M_total,K], a_scale[M_total,ceil(K/128)], B_T[G*N,K], b_scale[G*ceil(N/128),ceil(K/128)],
+ *                offsets[G+1] s32 (device; non-decreasing, any alignment) -> C[M_total,N]; rows outside
+ *                [offsets[0], offsets[G]) are not written                                                */
+#define PB200_K_FP8_GEMM         24
+#define PB200_K_FP8_GROUPED_GEMM 25
+
 /* ---- create-time flags -------------------------------------------------- */
 #define PB200_F_OUT_BF16       (1ull << 0)  /* round the output to bf16            */
 #define PB200_F_CAUSAL         (1ull << 1)  /* attention: lower-triangular mask    */
@@ -175,6 +220,8 @@ extern "C" {
 /* attention backward: the two-pass form (dQ in a pass of its own, no atomics, bit-reproducible);
  * the default forms dQ in the dK/dV pass and accumulates it across key tiles with fp32 atomics */
 #define PB200_F_DETERMINISTIC  (1ull << 7)
+#define PB200_F_IN_BF16        (1ull << 8)  /* the input of a quantising kernel is bf16   */
+#define PB200_F_IDS_S64        (1ull << 9)  /* moe route: expert ids are 64-bit integers  */
 
 /* Launch geometry of a handle, as the reference's Kernel object exposes it
  * (pyptx/kernel.py:402-447: grid, block, cluster, smem). */

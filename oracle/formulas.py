@@ -176,3 +176,94 @@ def max_scaled_err(out: torch.Tensor, ref: torch.Tensor) -> float:
     """``max |out-ref| / max(|ref|, 1)``, the elementwise companion of ``rel_fro``."""
     o, r = out.double().cpu(), ref.double().cpu()
     return float(((o - r).abs() / r.abs().clamp_min(1.0)).max())
+
+
+# ---- mixture-of-experts token movement and 8-bit block scaling (float64, plain loops) --------------
+# The reference has no counterpart; these restate the definitions in include/pyptx_b200.h.
+
+def moe_route_ref(ids: torch.Tensor, experts: int, block: int, rows: int):
+    """(row_of, entry_of, offsets) of the stable sort by expert; int32."""
+    flat = ids.reshape(-1).tolist()
+    lists: list[list[int]] = [[] for _ in range(experts)]
+    for i, e in enumerate(flat):
+        if 0 <= e < experts:
+            lists[e].append(i)
+    row_of, entry_of, offsets, at = [-1] * len(flat), [-1] * rows, [0], 0
+    for entries in lists:
+        for r, i in enumerate(entries, at):
+            if r < rows:
+                row_of[i], entry_of[r] = r, i
+        at += -(-len(entries) // block) * block
+        offsets.append(min(at, rows))
+    as_int = [torch.tensor(v, dtype=torch.int32) for v in (row_of, entry_of, offsets)]
+    return as_int[0].view(ids.shape), as_int[1], as_int[2]
+
+
+def moe_dispatch_ref(x: torch.Tensor, entry_of: torch.Tensor, top_k: int) -> torch.Tensor:
+    out = torch.zeros(entry_of.numel(), x.shape[1], dtype=x.dtype)
+    owned = entry_of >= 0
+    out[owned] = x[entry_of[owned].long() // top_k]
+    return out
+
+
+def moe_combine_ref(rows: torch.Tensor, weights: torch.Tensor | None, row_of: torch.Tensor):
+    """(sum, sum of magnitudes) in float64 of each token's weighted rows; weights None = 1."""
+    T, k = row_of.shape
+    out = torch.zeros(T, rows.shape[1], dtype=torch.float64)
+    mag = torch.zeros_like(out)
+    for j in range(k):
+        r = row_of[:, j].long()
+        part = rows[r.clamp_min(0)].double()
+        if weights is not None:
+            part = part * weights[:, j:j + 1].double()
+        part = torch.where((r >= 0)[:, None], part, torch.zeros_like(part))
+        out += part
+        mag += part.abs()
+    return out, mag
+
+
+def moe_combine_bwd_ref(rows: torch.Tensor, weights: torch.Tensor, row_of: torch.Tensor, dout: torch.Tensor):
+    """(d_rows, d_weights, magnitudes of d_weights' terms) in float64."""
+    T, k = row_of.shape
+    d_rows = torch.zeros(rows.shape, dtype=torch.float64)
+    d_w = torch.zeros(T, k, dtype=torch.float64)
+    mag = torch.zeros(T, k, dtype=torch.float64)
+    for j in range(k):
+        t = torch.nonzero(row_of[:, j] >= 0).view(-1)
+        r = row_of[t, j].long()
+        d_rows[r] = weights[t, j:j + 1].double() * dout[t].double()
+        terms = rows[r].double() * dout[t].double()
+        d_w[t, j], mag[t, j] = terms.sum(-1), terms.abs().sum(-1)
+    return d_rows, d_w, mag
+
+
+def e4m3_round(x: torch.Tensor) -> torch.Tensor:
+    """Nearest e4m3 value (ties to even, 448 at most) of float64 values: four significant bits, steps of
+    2^-9 at least.  NaN stays."""
+    _, e = torch.frexp(x)
+    step = torch.exp2((e - 4).clamp_min(-9).double())
+    return (torch.round(x / step) * step).clamp(-448.0, 448.0)
+
+
+def fp8_quantize_ref(x: torch.Tensor, block_rows: int):
+    """(q values, scale) of 128-column blocks: scale, reciprocal and product are f32 numbers, each
+    formed in float64 and rounded once; amax over the numbers of a block."""
+    M, K = x.shape
+    rb, cb = -(-M // block_rows), -(-K // 128)
+    v = torch.zeros(rb * block_rows, cb * 128, dtype=torch.float64)
+    v[:M, :K] = x.double()
+    v = v.view(rb, block_rows, cb, 128)
+    mag = torch.where(torch.isnan(v), torch.zeros_like(v), v.abs())
+    scale = (mag.amax(dim=(1, 3), keepdim=True) / 448.0).float().double().clamp_min(2.0 ** -120)
+    inv = (1.0 / scale).float().double()
+    q = e4m3_round((v * inv).float().double())
+    return q.view(rb * block_rows, cb * 128)[:M, :K], scale.view(rb, cb)
+
+
+def fp8_gemm_ref(a, a_scale, b, b_scale):
+    """(D, sum of magnitudes) in float64 of the block-scaled product of e4m3 tensors."""
+    M, K = a.shape
+    N = b.shape[0]
+    A = a.float().double() * a_scale.double().repeat_interleave(128, dim=1)[:, :K]
+    B = b.float().double() * b_scale.double().repeat_interleave(128, dim=0)[:N].repeat_interleave(128, dim=1)[:, :K]
+    return A @ B.T, A.abs() @ B.abs().T

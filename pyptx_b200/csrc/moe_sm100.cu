@@ -1,0 +1,792 @@
+// Mixture-of-experts token movement for sm_100a, around the grouped GEMMs:
+//   route      expert ids -> a stable sort of the T*k entries by expert (both directions of the map
+//              and the experts' row offsets, padded to the grouped kernels' row blocks)
+//   dispatch   tokens -> rows sorted by expert (rows as they are, or quantised to e4m3 with a scale
+//              for each 128 columns), and its gradient
+//   combine    rows -> tokens, weighted, and its gradient
+// and the quantisation of plain matrices that the 8-bit GEMM takes.
+//
+// Everything but the sort moves bytes and computes next to nothing, so those kernels are bound by
+// HBM: 16-byte accesses, consecutive lanes on consecutive segments, every independent load issued
+// before the first use, each input read once and each output written once.  No atomics: every sum
+// has a fixed order, so results are the same from run to run.
+#include "common.cuh"
+#include "ptx.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+namespace pb200 {
+namespace {
+
+constexpr int kThreads = 128;                 // movement kernels: 4 warps, one unit of work per warp
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTopK = 32;                  // one lane holds one choice's row and weight
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxBlock = 1024;
+constexpr int kScaleBlock = 128;
+
+__device__ __forceinline__ void pdl_prologue() {
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+}
+
+__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void st_stream(uint4* p, const uint4& v) {
+    asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};"
+                 :: "l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// A 16-byte vector as f32 values: 8 bf16 or 4 f32.
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
+        f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y);
+        f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+};
+template <> struct Vec<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<uint32_t*>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// ---------------------------------------------------------------------------
+// Route: a stable counting sort in one launch of one cluster.
+//
+// Entry i = t*k + j asks for expert ids[i].  CTA c of the cluster owns a contiguous range of
+// entries and each of its warps a contiguous part of that, so "earlier entry" is "earlier round of
+// the same warp, or an earlier warp, or an earlier CTA".  A warp walks its part 32 entries at a
+// time; match_any gives each lane its rank among the lanes with the same expert, and the warp's
+// running counters in shared memory the rest.  Counters are then prefix-summed over warps (each
+// thread one expert), over CTAs (through distributed shared memory) and, padded to `block` rows,
+// over experts; the row of an entry is the sum of the three.  Rows that no entry owns get entry -1
+// in the same launch, so nothing has to be cleared beforehand.
+//
+// Latency-bound: the ids are read once (4 or 8 bytes an entry), the maps written once.
+// ---------------------------------------------------------------------------
+constexpr int kRouteThreads = 1024;
+constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteRegRounds = 8;            // rounds whose ids and ranks stay in registers
+
+struct RouteArgs {
+    const void* ids;
+    int* row_of;
+    int* entry_of;
+    int* offsets;
+    int n;                // entries
+    int experts;
+    int block;
+    int rows;
+    int per_warp;         // entries of a warp, a multiple of 32
+};
+
+template <typename IdT>
+__device__ __forceinline__ int load_id(const void* ids, int i, int n, int experts) {
+    if (i >= n) return -1;
+    const IdT v = __ldg(reinterpret_cast<const IdT*>(ids) + i);
+    return v >= 0 && v < (IdT)experts ? (int)v : -1;      // ids outside [0, experts) are dropped
+}
+
+// Rank of this lane's entry among the entries of its expert that this warp has seen; advances the counter.
+__device__ __forceinline__ int warp_rank(int* counters, int id, int lane) {
+    const unsigned same = __match_any_sync(0xffffffffu, id);
+    const unsigned before = same & ((1u << lane) - 1u);
+    int base = 0;
+    if (id >= 0) base = counters[id];
+    __syncwarp();
+    if (id >= 0 && before == 0) counters[id] = base + __popc(same);
+    __syncwarp();
+    return base + __popc(before);
+}
+
+template <typename IdT, bool IN_REGS>
+__global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
+    pdl_prologue();
+    extern __shared__ int smem[];
+    const int E = a.experts;
+    int* counters = smem;                           // [warps][E]: counts, then prefix over warps
+    int* cta_count = counters + kRouteWarps * E;    // [E], read by the other CTAs
+    int* base = cta_count + E;                      // [E] first row of this CTA's entries of an expert
+    int* filled = base + E;                         // [E] end of the expert's entries (row)
+    int* ends = filled + E;                         // [E] end of the expert's rows
+    __shared__ int warp_total[kRouteWarps];
+
+    uint32_t n_ctas;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n_ctas));
+    const int rank = (int)ptx::cluster_ctarank();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int first = (rank * kRouteWarps + warp) * a.per_warp;
+    const int rounds = first < a.n ? (min(a.per_warp, a.n - first) + 31) / 32 : 0;
+
+    int my_id[kRouteRegRounds], my_rank[kRouteRegRounds];
+    if (IN_REGS) {
+#pragma unroll
+        for (int r = 0; r < kRouteRegRounds; ++r) my_id[r] = r < rounds ? load_id<IdT>(a.ids, first + r * 32 + lane, a.n, E) : -1;
+    }
+    for (int i = tid; i < kRouteWarps * E; i += kRouteThreads) counters[i] = 0;
+    __syncthreads();
+    if (IN_REGS) {
+#pragma unroll
+        for (int r = 0; r < kRouteRegRounds; ++r)
+            if (r < rounds) my_rank[r] = warp_rank(counters + warp * E, my_id[r], lane);
+    } else {
+        int next = load_id<IdT>(a.ids, first + lane, rounds > 0 ? a.n : 0, E);
+        for (int r = 0; r < rounds; ++r) {
+            const int i = first + r * 32 + lane, id = next;
+            next = r + 1 < rounds ? load_id<IdT>(a.ids, i + 32, a.n, E) : -1;
+            const int rk = warp_rank(counters + warp * E, id, lane);
+            if (i < a.n) a.row_of[i] = rk;          // kept for the second pass of this same thread
+        }
+    }
+    __syncthreads();
+    // prefix over warps: counters[w][e] = entries of e in earlier warps of this CTA
+    for (int e = tid; e < E; e += kRouteThreads) {
+        int run = 0;
+#pragma unroll 8
+        for (int w = 0; w < kRouteWarps; ++w) {
+            const int c = counters[w * E + e];
+            counters[w * E + e] = run;
+            run += c;
+        }
+        cta_count[e] = run;
+    }
+    if (n_ctas > 1) ptx::cluster_sync_all(); else __syncthreads();
+    // totals over CTAs, then a block-wide exclusive prefix of the padded totals (E <= 1024 threads)
+    int total = 0, before = 0;
+    if (tid < E) {
+        const uint32_t own = ptx::smem_u32(cta_count + tid);
+        for (int c = 0; c < (int)n_ctas; ++c) {
+            int v;
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ptx::map_to_cta(own, (uint32_t)c)) : "memory");
+            if (c < rank) before += v;
+            total += v;
+        }
+    }
+    const int padded = (total + a.block - 1) / a.block * a.block;
+    int incl = padded;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_total[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        int v = warp_total[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        warp_total[lane] = v;
+    }
+    __syncthreads();
+    const int end = incl + (warp > 0 ? warp_total[warp - 1] : 0);
+    if (tid < E) {
+        const int start = end - padded;
+        base[tid] = start + before;
+        filled[tid] = start + total;
+        ends[tid] = end;
+        if (rank == 0) {
+            a.offsets[tid + 1] = min(end, a.rows);
+            if (tid == 0) a.offsets[0] = 0;
+        }
+    }
+    __syncthreads();
+    // entries
+    auto place = [&](int i, int id, int rk) {
+        int row = -1;
+        if (id >= 0) {
+            row = base[id] + counters[warp * E + id] + rk;
+            if (row < a.rows) a.entry_of[row] = i; else row = -1;      // no room: dropped
+        }
+        a.row_of[i] = row;
+    };
+    if (IN_REGS) {
+#pragma unroll
+        for (int r = 0; r < kRouteRegRounds; ++r) {
+            const int i = first + r * 32 + lane;
+            if (r < rounds && i < a.n) place(i, my_id[r], my_rank[r]);
+        }
+    } else {
+#pragma unroll 4
+        for (int r = 0; r < rounds; ++r) {
+            const int i = first + r * 32 + lane;
+            if (i < a.n) place(i, load_id<IdT>(a.ids, i, a.n, E), a.row_of[i]);
+        }
+    }
+    // rows without an entry: each expert's padding, then everything behind the last expert
+    for (int e = rank * kRouteWarps + warp; e < E; e += (int)n_ctas * kRouteWarps)
+        for (int r = filled[e] + lane; r < min(ends[e], a.rows); r += 32) a.entry_of[r] = -1;
+    for (int r = ends[E - 1] + rank * kRouteThreads + tid; r < a.rows; r += (int)n_ctas * kRouteThreads) a.entry_of[r] = -1;
+    if (n_ctas > 1) ptx::cluster_sync_all();        // shared memory must outlive the other CTAs' reads
+}
+
+// ---------------------------------------------------------------------------
+// Zero rows.  A unit is 32 rows x one segment: a lane looks at one row, the warp then clears its
+// segment of every row that no entry owns.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void zero_unowned(uint4* out, const int* __restrict__ entry_of, int64_t row0, int rows, int vecs,
+                                             int vec0, int vec1, int lane) {
+    const int64_t r = row0 + lane;
+    unsigned todo = __ballot_sync(0xffffffffu, r < rows && __ldg(entry_of + r) < 0);
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    while (todo) {
+        const int b = __ffs(todo) - 1;
+        todo &= todo - 1;
+        uint4* dst = out + (row0 + b) * vecs;
+        for (int v = vec0 + lane; v < vec1; v += 32) st_stream(dst + v, zero);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Dispatch: a warp reads U x 512 bytes of one token once and writes them to its k rows.  In token
+// order the tokens are read once from HBM; in row order they would be read k times.
+// ---------------------------------------------------------------------------
+struct MoveArgs {
+    const void* src;              // tokens (dispatch) or rows (combine)
+    const int* row_of;
+    const int* entry_of;
+    const float* weights;
+    void* dst;
+    float* dst_scale;
+    const void* grad;
+    void* d_rows;
+    float* d_weights;
+    int64_t tokens;
+    int64_t zero_units;           // units before the tokens' ones
+    int top_k;
+    int rows;
+    int vecs;                     // 16-byte vectors of a row
+    int segs;                     // segments of a row
+    int width;                    // columns
+    int scale_cols;
+};
+
+template <int U>
+__global__ void __launch_bounds__(kThreads) dispatch_kernel(MoveArgs a) {
+    pdl_prologue();
+    const int lane = threadIdx.x & 31;
+    int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    uint4* out = reinterpret_cast<uint4*>(a.dst);
+    if (unit < a.zero_units) {
+        const int seg = (int)(unit % a.segs);
+        zero_unowned(out, a.entry_of, unit / a.segs * 32, a.rows, a.vecs, seg * 32 * U, min(a.vecs, (seg + 1) * 32 * U), lane);
+        return;
+    }
+    unit -= a.zero_units;
+    const int64_t t = unit / a.segs;
+    if (t >= a.tokens) return;
+    const int v0 = (int)(unit - t * a.segs) * 32 * U + lane;
+    const uint4* x = reinterpret_cast<const uint4*>(a.src) + t * a.vecs;
+    const int my_row = lane < a.top_k ? __ldg(a.row_of + t * a.top_k + lane) : -1;
+    uint4 d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (v0 + 32 * u < a.vecs) d[u] = ld_stream(x + v0 + 32 * u);
+    for (int j = 0; j < a.top_k; ++j) {
+        const int r = __shfl_sync(0xffffffffu, my_row, j);
+        if (r < 0 || r >= a.rows) continue;
+        uint4* dst = out + (int64_t)r * a.vecs;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (v0 + 32 * u < a.vecs) st_stream(dst + v0 + 32 * u, d[u]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Quantisation of 128-column blocks: s = max(amax / 448, 2^-120), q = e4m3(x * (1 / s)), in f32 with
+// every step rounded to nearest.  2^-120 keeps 1/s finite, so that an all-zero block gives zeros.
+// amax ignores NaN: a NaN stays in its own element; an infinity makes its block's products NaN.
+// A lane holds 8 columns, 16 lanes a block, a warp two blocks.
+// ---------------------------------------------------------------------------
+constexpr float kFp8Max = 448.0f;
+
+__device__ __forceinline__ float block_scale(float amax) {
+    return fmaxf(__fdiv_rn(amax, kFp8Max), 0x1p-120f);
+}
+__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float inv) {
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        h[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * inv, v[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+// 8 consecutive columns; columns come in multiples of 16, so 8 of them are all there or not at all.
+template <typename T> __device__ __forceinline__ void load8(const T* p, bool there, float (&v)[8]);
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, bool there, float (&v)[8]) {
+    Vec<__nv_bfloat16>::unpack(there ? ld_stream(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0), v);
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, bool there, float (&v)[8]) {
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    const uint4 lo = there ? ld_stream(reinterpret_cast<const uint4*>(p)) : z;
+    const uint4 hi = there ? ld_stream(reinterpret_cast<const uint4*>(p) + 1) : z;
+    float a[4], b[4];
+    Vec<float>::unpack(lo, a);
+    Vec<float>::unpack(hi, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+}
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+    return m;
+}
+__device__ __forceinline__ float amax_of_16_lanes(float m) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+
+// Rows quantised for each 1 x 128 block.  ROUTED: token t goes to its k rows, and rows that no entry
+// owns become zeros with scale 0; otherwise row t goes to row t.  A warp takes U x 256 columns.
+template <typename T, int U, bool ROUTED>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(MoveArgs a) {
+    pdl_prologue();
+    const int lane = threadIdx.x & 31;
+    int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    uint8_t* q_out = reinterpret_cast<uint8_t*>(a.dst);
+    if (ROUTED) {
+        if (unit < a.zero_units) {
+            const int seg = (int)(unit % a.segs);
+            const int64_t row0 = unit / a.segs * 32;
+            zero_unowned(reinterpret_cast<uint4*>(q_out), a.entry_of, row0, a.rows, a.vecs, seg * 16 * U,
+                         min(a.vecs, (seg + 1) * 16 * U), lane);
+            const int64_t r = row0 + lane;
+            if (r < a.rows && __ldg(a.entry_of + r) < 0)
+                for (int c = seg * 2 * U; c < min(a.scale_cols, (seg + 1) * 2 * U); ++c) a.dst_scale[r * a.scale_cols + c] = 0.0f;
+            return;
+        }
+        unit -= a.zero_units;
+    }
+    const int64_t t = unit / a.segs;
+    if (t >= a.tokens) return;
+    const int c0 = (int)(unit - t * a.segs) * 256 * U + lane * 8;
+    const T* x = reinterpret_cast<const T*>(a.src) + t * a.width;
+    int my_row = -1;
+    if (ROUTED && lane < a.top_k) my_row = __ldg(a.row_of + t * a.top_k + lane);
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load8<T>(x + c0 + 256 * u, c0 + 256 * u < a.width, v[u]);
+    uint2 q[U];
+    float scale[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        scale[u] = block_scale(amax_of_16_lanes(amax8(v[u])));
+        q[u] = quantize8(v[u], __frcp_rn(scale[u]));
+    }
+    const int n_dst = ROUTED ? a.top_k : 1;
+    for (int j = 0; j < n_dst; ++j) {
+        const int64_t r = ROUTED ? (int64_t)__shfl_sync(0xffffffffu, my_row, j) : t;
+        if (ROUTED && (r < 0 || r >= a.rows)) continue;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = c0 + 256 * u;
+            if (c < a.width) {
+                __stcs(reinterpret_cast<uint2*>(q_out + r * a.width + c), q[u]);
+                if ((lane & 15) == 0) a.dst_scale[r * a.scale_cols + c / kScaleBlock] = scale[u];
+            }
+        }
+    }
+}
+
+// 128 x 128 blocks (weights): a CTA of 256 threads holds one block, 8 rows x 8 columns a thread.
+constexpr int kBlockThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kBlockThreads) quantize_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                                        float* __restrict__ scales, int64_t rows, int cols,
+                                                                        int scale_cols) {
+    pdl_prologue();
+    __shared__ float part[kBlockThreads / 32];
+    const int64_t row0 = (int64_t)(blockIdx.x / scale_cols) * kScaleBlock + threadIdx.x / 16;
+    const int col = (int)(blockIdx.x % scale_cols) * kScaleBlock + (threadIdx.x % 16) * 8;
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) load8<T>(x + (row0 + 16 * i) * cols + col, row0 + 16 * i < rows && col < cols, v[i]);
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, amax8(v[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x / 32] = m;
+    __syncthreads();
+    m = part[0];
+#pragma unroll
+    for (int i = 1; i < kBlockThreads / 32; ++i) m = fmaxf(m, part[i]);
+    const float scale = block_scale(m), inv = __frcp_rn(scale);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (row0 + 16 * i < rows && col < cols)
+            __stcs(reinterpret_cast<uint2*>(q + (row0 + 16 * i) * cols + col), quantize8(v[i], inv));
+    if (threadIdx.x == 0) scales[blockIdx.x] = scale;
+}
+
+// ---------------------------------------------------------------------------
+// Combine: out[t] = sum_j weights[t,j] * rows[row_of[t,j]], f32 sums in the order of j, rounded once.
+// Without weights it is the gradient of dispatch.  A warp takes U x 512 bytes of one token and keeps
+// four rows' loads in flight.
+// ---------------------------------------------------------------------------
+template <typename T, int U, bool WEIGHTED>
+__global__ void __launch_bounds__(kThreads) combine_kernel(MoveArgs a) {
+    pdl_prologue();
+    constexpr int N = Vec<T>::kN;
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int64_t t = unit / a.segs;
+    if (t >= a.tokens) return;
+    const int v0 = (int)(unit - t * a.segs) * 32 * U + lane;
+    const uint4* rows = reinterpret_cast<const uint4*>(a.src);
+    int my_row = -1;
+    float my_w = 1.0f;
+    if (lane < a.top_k) {
+        my_row = __ldg(a.row_of + t * a.top_k + lane);
+        if (WEIGHTED) my_w = __ldg(a.weights + t * a.top_k + lane);
+    }
+    if (my_row >= a.rows) my_row = -1;
+    float acc[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[u][i] = 0.0f;
+    constexpr int kGroup = 4;
+    for (int j0 = 0; j0 < a.top_k; j0 += kGroup) {
+        uint4 d[kGroup][U];
+        int r[kGroup];
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+            r[g] = j0 + g < a.top_k ? __shfl_sync(0xffffffffu, my_row, j0 + g) : -1;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (r[g] >= 0 && v0 + 32 * u < a.vecs) d[g][u] = ld_stream(rows + (int64_t)r[g] * a.vecs + v0 + 32 * u);
+        }
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+            if (r[g] < 0) continue;
+            const float w = WEIGHTED ? __shfl_sync(0xffffffffu, my_w, j0 + g) : 1.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float f[N];
+                Vec<T>::unpack(d[g][u], f);
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[u][i] = WEIGHTED ? fmaf(w, f[i], acc[u][i]) : acc[u][i] + f[i];
+            }
+        }
+    }
+    uint4* out = reinterpret_cast<uint4*>(a.dst) + t * a.vecs;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (v0 + 32 * u < a.vecs) st_stream(out + v0 + 32 * u, Vec<T>::pack(acc[u]));
+}
+
+// ---------------------------------------------------------------------------
+// Combine backward: d_rows[r] = weights[t,j] * grad[t] (zeros where no entry owns r) and
+// d_weights[t,j] = <rows[r], grad[t]>.  A CTA takes one token: its gradient is read once and held in
+// registers while the k rows stream by.  Partial dot products go lane -> warp (shuffles) -> CTA
+// (shared memory, one slot for each warp and choice), always in the same order.
+// ---------------------------------------------------------------------------
+template <typename T, int U>
+__global__ void __launch_bounds__(kThreads) combine_bwd_kernel(MoveArgs a) {
+    pdl_prologue();
+    constexpr int N = Vec<T>::kN;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint4* d_rows = reinterpret_cast<uint4*>(a.d_rows);
+    const int64_t zero_blocks = (a.zero_units + kWarps - 1) / kWarps;
+    if (blockIdx.x < zero_blocks) {
+        const int64_t unit = (int64_t)blockIdx.x * kWarps + warp;
+        if (unit < a.zero_units) {
+            const int seg = (int)(unit % a.segs);
+            zero_unowned(d_rows, a.entry_of, unit / a.segs * 32, a.rows, a.vecs, seg * 128, min(a.vecs, (seg + 1) * 128), lane);
+        }
+        return;
+    }
+    __shared__ float part[kMaxTopK][kWarps];
+    const int64_t t = (int64_t)blockIdx.x - zero_blocks;
+    const uint4* grad = reinterpret_cast<const uint4*>(a.grad) + t * a.vecs;
+    const uint4* rows = reinterpret_cast<const uint4*>(a.src);
+    int my_row = -1;
+    float my_w = 0.0f;
+    if (lane < a.top_k) {
+        my_row = __ldg(a.row_of + t * a.top_k + lane);
+        my_w = __ldg(a.weights + t * a.top_k + lane);
+    }
+    if (my_row >= a.rows) my_row = -1;
+    for (int j = lane; j < a.top_k; j += 32) part[j][warp] = 0.0f;
+    __syncwarp();
+    for (int base = 0; base < a.vecs; base += kThreads * U) {
+        const int v0 = base + threadIdx.x;
+        uint4 graw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            graw[u] = v0 + kThreads * u < a.vecs ? ld_stream(grad + v0 + kThreads * u) : make_uint4(0, 0, 0, 0);
+        float g[U][N];
+#pragma unroll
+        for (int u = 0; u < U; ++u) Vec<T>::unpack(graw[u], g[u]);
+        for (int j = 0; j < a.top_k; ++j) {
+            const int r = __shfl_sync(0xffffffffu, my_row, j);
+            if (r < 0) continue;
+            const float w = __shfl_sync(0xffffffffu, my_w, j);
+            uint4 d[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (v0 + kThreads * u < a.vecs) d[u] = ld_stream(rows + (int64_t)r * a.vecs + v0 + kThreads * u);
+            float dot = 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (v0 + kThreads * u >= a.vecs) continue;
+                float f[N], o[N];
+                Vec<T>::unpack(d[u], f);
+#pragma unroll
+                for (int i = 0; i < N; ++i) { dot = fmaf(f[i], g[u][i], dot); o[i] = w * g[u][i]; }
+                st_stream(d_rows + (int64_t)r * a.vecs + v0 + kThreads * u, Vec<T>::pack(o));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            if (lane == 0) part[j][warp] += dot;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < a.top_k) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) s += part[threadIdx.x][w];
+        a.d_weights[t * a.top_k + threadIdx.x] = s;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int route_ctas(int64_t n) {
+    // One CTA ranks 32 entries a warp and round; a second CTA costs a cluster barrier, so the cluster
+    // grows only once a CTA would walk more than two rounds.
+    int ctas = 1;
+    while (ctas < 8 && n > (int64_t)ctas * 2 * kRouteThreads) ctas *= 2;
+    return ctas;
+}
+size_t route_smem(int64_t experts) { return (size_t)(kRouteWarps + 4) * experts * sizeof(int); }
+
+bool is_bf16(const Record& r) { return (r.flags & PB200_F_OUT_BF16) != 0; }
+
+// Units of a movement kernel: U vectors a lane when that still gives every SM sub-partition a few
+// warps, else one (short calls are bound by latency, long ones by bytes in flight).
+bool few_units(int64_t units_at_one) { return units_at_one < (int64_t)sm_count() * 16; }
+
+template <typename... KArgs, typename... Args>
+int enqueue(const char* what, void (*kernel)(KArgs...), int64_t grid, int threads, cudaStream_t stream, char* err, Args... args) {
+    cudaError_t e = launch_with_pdl(kernel, dim3((unsigned)grid), dim3(threads), 0, stream, args...);
+    if (e != cudaSuccess) { set_err(err, "%s launch failed: %s", what, cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
+    return PB200_OK;
+}
+
+template <typename IdT>
+int launch_route(const Record& r, cudaStream_t stream, void** p, char* err) {
+    RouteArgs a;
+    a.ids = p[0];
+    a.row_of = (int*)p[1];
+    a.entry_of = (int*)p[2];
+    a.offsets = (int*)p[3];
+    const int64_t n = r.dims[0] * r.dims[1];
+    a.n = (int)n;
+    a.experts = (int)r.dims[2];
+    a.block = (int)r.dims[3];
+    a.rows = (int)r.dims[4];
+    const int ctas = (int)r.geom.cluster[0];
+    a.per_warp = (int)(ceil_div(ceil_div(n, ctas * kRouteWarps), 32) * 32);
+    auto kernel = a.per_warp <= 32 * kRouteRegRounds ? route_kernel<IdT, true> : route_kernel<IdT, false>;
+    const size_t smem = route_smem(a.experts);
+    cudaError_t e = cudaSuccess;
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(ctas);
+        cfg.blockDim = dim3(kRouteThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)ctas;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        e = cudaLaunchKernelEx(&cfg, kernel, a);
+    }
+    if (e != cudaSuccess) { set_err(err, "moe_route launch failed: %s", cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
+    return PB200_OK;
+}
+
+MoveArgs move_args(const Record& r, int64_t width, int elt_bytes) {
+    MoveArgs a{};
+    a.tokens = r.dims[0];
+    a.top_k = (int)r.dims[1];
+    a.rows = (int)r.dims[2];
+    a.width = (int)width;
+    a.vecs = (int)(width * elt_bytes / 16);
+    a.scale_cols = (int)ceil_div(width, kScaleBlock);
+    return a;
+}
+
+template <typename T, bool ROUTED>
+int launch_quantize_rows(MoveArgs a, cudaStream_t stream, char* err) {
+    const bool few = few_units(a.tokens * ceil_div(a.width, 1024));
+    const int u = few ? 1 : 4;
+    a.segs = (int)ceil_div(a.width, 256 * u);
+    a.zero_units = ROUTED ? ceil_div(a.rows, 32) * a.segs : 0;
+    const int64_t grid = ceil_div(a.zero_units + a.tokens * a.segs, kWarps);
+    return enqueue("fp8 quantisation", few ? quantize_rows_kernel<T, 1, ROUTED> : quantize_rows_kernel<T, 4, ROUTED>, grid, kThreads,
+                   stream, err, a);
+}
+
+template <typename T, bool WEIGHTED>
+int launch_combine(MoveArgs a, cudaStream_t stream, char* err) {
+    const bool few = few_units(a.tokens * ceil_div(a.vecs, 64));
+    a.segs = (int)ceil_div(a.vecs, few ? 32 : 64);
+    return enqueue("moe_combine", few ? combine_kernel<T, 1, WEIGHTED> : combine_kernel<T, 2, WEIGHTED>,
+                   ceil_div(a.tokens * a.segs, kWarps), kThreads, stream, err, a);
+}
+
+}  // namespace
+
+int plan_moe(Record& r, char* err) {
+    auto bad = [&](const char* what) { set_err(err, "%s", what); return PB200_ERR_BAD_SHAPE; };
+    pb200_geometry& g = r.geom;
+    for (int i = 0; i < 3; ++i) g.grid[i] = g.block[i] = g.cluster[i] = 1;
+    g.block[0] = kThreads;
+    const int need = r.kernel_id == PB200_K_FP8_QUANTIZE ? 3 : r.kernel_id == PB200_K_MOE_ROUTE ? 5 : 4;
+    if (r.n_dims != need) { set_err(err, "kernel %d needs %d dims, got %d", r.kernel_id, need, r.n_dims); return PB200_ERR_BAD_SHAPE; }
+    for (int i = 0; i < need; ++i) {
+        if (r.dims[i] < 1) return bad("all sizes must be positive");
+        if (r.dims[i] > 0x7fffffffLL) return bad("extent exceeds 2^31-1");
+    }
+    if (r.kernel_id == PB200_K_FP8_QUANTIZE) {
+        const int64_t M = r.dims[0], K = r.dims[1];
+        if (K % 16 != 0) { set_err(err, "K=%lld must be divisible by 16", (long long)K); return PB200_ERR_BAD_SHAPE; }
+        if (r.dims[2] != 1 && r.dims[2] != kScaleBlock) return bad("block_rows must be 1 or 128");
+        const int64_t grid = r.dims[2] == 1 ? ceil_div(M * ceil_div(K, 256), kWarps) : ceil_div(M, kScaleBlock) * ceil_div(K, kScaleBlock);
+        if (grid > 0x7fffffffLL) return bad("matrix is too large for one launch");
+        g.grid[0] = (uint32_t)grid;
+        if (r.dims[2] != 1) g.block[0] = kBlockThreads;
+        g.n_inputs = 1;
+        g.n_outputs = 2;
+        return PB200_OK;
+    }
+    const int64_t T = r.dims[0], k = r.dims[1];
+    if (k > kMaxTopK) { set_err(err, "top_k=%lld exceeds %d", (long long)k, kMaxTopK); return PB200_ERR_BAD_SHAPE; }
+    if (T * k > (1LL << 30)) return bad("tokens * top_k exceeds 2^30");
+    if (r.kernel_id == PB200_K_MOE_ROUTE) {
+        const int64_t E = r.dims[2], block = r.dims[3], rows = r.dims[4];
+        if (E > kMaxExperts) { set_err(err, "E=%lld exceeds %d", (long long)E, kMaxExperts); return PB200_ERR_BAD_SHAPE; }
+        if (block > kMaxBlock) { set_err(err, "block=%lld exceeds %d", (long long)block, kMaxBlock); return PB200_ERR_BAD_SHAPE; }
+        if (rows % block != 0) { set_err(err, "rows=%lld must be divisible by block=%lld", (long long)rows, (long long)block); return PB200_ERR_BAD_SHAPE; }
+        g.cluster[0] = g.grid[0] = (uint32_t)route_ctas(T * k);
+        g.block[0] = kRouteThreads;
+        g.smem_bytes = (uint32_t)route_smem(E);
+        g.n_inputs = 1;
+        g.n_outputs = 3;
+        return PB200_OK;
+    }
+    const int64_t rows = r.dims[2], H = r.dims[3];
+    const bool fp8 = r.kernel_id == PB200_K_MOE_DISPATCH_FP8;
+    const int unit = fp8 ? 16 : is_bf16(r) ? 8 : 4;
+    if (H % unit != 0) { set_err(err, "H=%lld must be divisible by %d", (long long)H, unit); return PB200_ERR_BAD_SHAPE; }
+    // one warp for each 32 vectors at most, and the same again for rows to clear
+    if (ceil_div(T + ceil_div(rows, 32), 1) * ceil_div(H, 128) > 0x7fffffffLL) return bad("tensor is too large for one launch");
+    g.grid[0] = (uint32_t)ceil_div(T * ceil_div(H, 128), kWarps);
+    switch (r.kernel_id) {
+        case PB200_K_MOE_DISPATCH:     g.n_inputs = 3; g.n_outputs = 1; break;
+        case PB200_K_MOE_DISPATCH_FP8: g.n_inputs = 3; g.n_outputs = 2; break;
+        case PB200_K_MOE_DISPATCH_BWD: g.n_inputs = 2; g.n_outputs = 1; break;
+        case PB200_K_MOE_COMBINE:      g.n_inputs = 3; g.n_outputs = 1; break;
+        default:                       g.n_inputs = 5; g.n_outputs = 2; break;
+    }
+    return PB200_OK;
+}
+
+int launch_moe(const Record& r, cudaStream_t stream, void** p, char* err) {
+    const bool b16 = is_bf16(r), in_b16 = (r.flags & PB200_F_IN_BF16) != 0;
+    switch (r.kernel_id) {
+    case PB200_K_MOE_ROUTE:
+        return (r.flags & PB200_F_IDS_S64) ? launch_route<int64_t>(r, stream, p, err) : launch_route<int32_t>(r, stream, p, err);
+    case PB200_K_MOE_DISPATCH: {
+        MoveArgs a = move_args(r, r.dims[3], b16 ? 2 : 4);
+        a.src = p[0]; a.row_of = (const int*)p[1]; a.entry_of = (const int*)p[2]; a.dst = p[3];
+        const bool few = few_units(a.tokens * ceil_div(a.vecs, 128));
+        a.segs = (int)ceil_div(a.vecs, few ? 32 : 128);
+        a.zero_units = ceil_div(a.rows, 32) * a.segs;
+        return enqueue("moe_dispatch", few ? dispatch_kernel<1> : dispatch_kernel<4>,
+                       ceil_div(a.zero_units + a.tokens * a.segs, kWarps), kThreads, stream, err, a);
+    }
+    case PB200_K_MOE_DISPATCH_FP8: {
+        MoveArgs a = move_args(r, r.dims[3], 1);
+        a.src = p[0]; a.row_of = (const int*)p[1]; a.entry_of = (const int*)p[2]; a.dst = p[3]; a.dst_scale = (float*)p[4];
+        return in_b16 ? launch_quantize_rows<__nv_bfloat16, true>(a, stream, err) : launch_quantize_rows<float, true>(a, stream, err);
+    }
+    case PB200_K_MOE_DISPATCH_BWD: {
+        MoveArgs a = move_args(r, r.dims[3], b16 ? 2 : 4);
+        a.row_of = (const int*)p[0]; a.src = p[1]; a.dst = p[2];
+        return b16 ? launch_combine<__nv_bfloat16, false>(a, stream, err) : launch_combine<float, false>(a, stream, err);
+    }
+    case PB200_K_MOE_COMBINE: {
+        MoveArgs a = move_args(r, r.dims[3], b16 ? 2 : 4);
+        a.src = p[0]; a.weights = (const float*)p[1]; a.row_of = (const int*)p[2]; a.dst = p[3];
+        return b16 ? launch_combine<__nv_bfloat16, true>(a, stream, err) : launch_combine<float, true>(a, stream, err);
+    }
+    case PB200_K_MOE_COMBINE_BWD: {
+        MoveArgs a = move_args(r, r.dims[3], b16 ? 2 : 4);
+        a.src = p[0]; a.weights = (const float*)p[1]; a.row_of = (const int*)p[2]; a.entry_of = (const int*)p[3]; a.grad = p[4];
+        a.d_rows = p[5]; a.d_weights = (float*)p[6];
+        a.segs = (int)ceil_div(a.vecs, 128);
+        a.zero_units = ceil_div(a.rows, 32) * a.segs;
+        const int64_t grid = ceil_div(a.zero_units, kWarps) + a.tokens;
+        return b16 ? enqueue("moe_combine_bwd", combine_bwd_kernel<__nv_bfloat16, 4>, grid, kThreads, stream, err, a)
+                   : enqueue("moe_combine_bwd", combine_bwd_kernel<float, 4>, grid, kThreads, stream, err, a);
+    }
+    default: break;
+    }
+    // PB200_K_FP8_QUANTIZE
+    const int64_t M = r.dims[0], K = r.dims[1];
+    if (r.dims[2] == 1) {
+        MoveArgs a{};
+        a.tokens = M; a.width = (int)K; a.scale_cols = (int)ceil_div(K, kScaleBlock);
+        a.src = p[0]; a.dst = p[1]; a.dst_scale = (float*)p[2];
+        return in_b16 ? launch_quantize_rows<__nv_bfloat16, false>(a, stream, err) : launch_quantize_rows<float, false>(a, stream, err);
+    }
+    const int sc = (int)ceil_div(K, kScaleBlock);
+    const int64_t grid = ceil_div(M, kScaleBlock) * sc;
+    if (in_b16)
+        return enqueue("fp8 quantisation", quantize_blocks_kernel<__nv_bfloat16>, grid, kBlockThreads, stream, err,
+                       (const __nv_bfloat16*)p[0], (uint8_t*)p[1], (float*)p[2], M, (int)K, sc);
+    return enqueue("fp8 quantisation", quantize_blocks_kernel<float>, grid, kBlockThreads, stream, err, (const float*)p[0],
+                   (uint8_t*)p[1], (float*)p[2], M, (int)K, sc);
+}
+
+}  // namespace pb200

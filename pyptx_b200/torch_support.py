@@ -51,7 +51,7 @@ _PTX_TO_TORCH_NAME = {
     "f16": "float16", "bf16": "bfloat16", "f32": "float32", "f64": "float64",
     "s8": "int8", "s16": "int16", "s32": "int32", "s64": "int64",
     "u8": "uint8", "b8": "uint8", "b16": "uint16", "b32": "uint32", "b64": "uint64",
-    "pred": "bool",
+    "pred": "bool", "e4m3": "float8_e4m3fn",
 }
 
 
@@ -69,7 +69,7 @@ def _torch_dtype_to_ptx_type_name(torch_dtype) -> str:
     table = {
         torch.float16: "f16", torch.bfloat16: "bf16", torch.float32: "f32", torch.float64: "f64",
         torch.int8: "s8", torch.int16: "s16", torch.int32: "s32", torch.int64: "s64",
-        torch.uint8: "u8", torch.bool: "pred",
+        torch.uint8: "u8", torch.bool: "pred", torch.float8_e4m3fn: "e4m3",
     }
     if torch_dtype not in table:
         raise TypeError(f"Cannot map torch dtype {torch_dtype} to a pyptx type")
@@ -106,7 +106,8 @@ class _Launcher:
         # c10::ScalarType integers, as the reference passes them (pyptx/torch_support.py:209-214)
         torch = _torch()
         codes = {torch.uint8: 0, torch.int8: 1, torch.int16: 2, torch.int32: 3, torch.int64: 4,
-                 torch.float16: 5, torch.float32: 6, torch.float64: 7, torch.bool: 11, torch.bfloat16: 15}
+                 torch.float16: 5, torch.float32: 6, torch.float64: 7, torch.bool: 11, torch.bfloat16: 15,
+                 torch.float8_e4m3fn: 24}
         self.out_dtype_codes = [codes[d] for d in self.out_dtypes]
         self.handle_int = int(kernel.handle)
 
