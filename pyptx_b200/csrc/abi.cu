@@ -51,6 +51,7 @@ bool is_gemm(int32_t k) {
            k == PB200_K_GROUPED_GEMM_SWIGLU || k == PB200_K_GROUPED_GEMM_VARLEN || k == PB200_K_GEMM_PUSH;
 }
 bool is_moe(int32_t k) { return k >= PB200_K_MOE_ROUTE && k <= PB200_K_FP8_QUANTIZE; }
+bool is_fp8_gemm(int32_t k) { return k == PB200_K_FP8_GEMM || k == PB200_K_FP8_GROUPED_GEMM; }
 
 // Handles whose buffers were already checked against the current device.
 std::mutex g_checked_mu;
@@ -176,6 +177,7 @@ PB200_API int64_t pb200_create(int32_t kernel_id, const int64_t* dims, size_t n_
     else if (kernel_id == PB200_K_FLASH_ATTN) rc = plan_attention(r, err_out);
     else if (kernel_id == PB200_K_FLASH_ATTN_BWD) rc = plan_attention_bwd(r, err_out);
     else if (is_moe(kernel_id)) rc = plan_moe(r, err_out);
+    else if (is_fp8_gemm(kernel_id)) rc = plan_fp8_gemm(r, err_out);
     else if (kernel_id == PB200_K_PEER_BARRIER) rc = plan_peer_barrier(r, err_out);
     else { set_err(err_out, "unknown kernel id %d", kernel_id); return PB200_ERR_BAD_KERNEL; }
     if (rc != PB200_OK) return rc;
@@ -215,6 +217,7 @@ PB200_API int pb200_launch_raw(int64_t handle, uint64_t stream, void** buffer_pt
     if (is_row(r.kernel_id)) return launch_row(r, s, buffer_ptrs, err_out);
     if (is_row_bwd(r.kernel_id)) return launch_row_bwd(r, s, buffer_ptrs, err_out);
     if (is_gemm(r.kernel_id)) return launch_gemm(r, s, buffer_ptrs, err_out);
+    if (is_fp8_gemm(r.kernel_id)) return launch_fp8_gemm(r, s, buffer_ptrs, err_out);
     if (is_moe(r.kernel_id)) return launch_moe(r, s, buffer_ptrs, err_out);
     if (r.kernel_id == PB200_K_PEER_BARRIER) return launch_peer_barrier(r, s, buffer_ptrs, err_out);
     if (r.kernel_id == PB200_K_FLASH_ATTN_BWD) return launch_attention_bwd(r, s, buffer_ptrs, err_out);

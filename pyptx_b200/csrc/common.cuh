@@ -61,6 +61,9 @@ int launch_attention_bwd(const Record& r, cudaStream_t stream, void** ptrs, char
 int plan_moe(Record& r, char* err);
 int launch_moe(const Record& r, cudaStream_t stream, void** ptrs, char* err);
 
+int plan_fp8_gemm(Record& r, char* err);
+int launch_fp8_gemm(const Record& r, cudaStream_t stream, void** ptrs, char* err);
+
 // Device-side status word (defined in abi.cu's translation unit of the same
 // library; each .cu that needs it reaches it through report_timeout()).
 // Layout: [0] = code (0 ok), [1] = kernel id, [2] = wait site, [3] = block id.

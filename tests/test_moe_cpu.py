@@ -7,7 +7,7 @@ import torch
 from oracle import formulas
 from pyptx_b200 import _ids, _native
 from pyptx_b200.examples.blackwell import moe
-from pyptx_b200.examples.blackwell.fp8_gemm import build_fp8_quantize
+from pyptx_b200.examples.blackwell.fp8_gemm import build_fp8_gemm, build_fp8_grouped_gemm_varlen, build_fp8_quantize
 from pyptx_b200.types import bf16, e4m3, f16, f32, s32, s64
 
 
@@ -107,3 +107,41 @@ def test_cpu_tensors_are_refused():
 def test_oracle_e4m3_rounding_matches_torch():
     x = torch.cat([torch.randn(4000) * 100, torch.randn(4000) * 0.01, torch.arange(-450, 450).float()]).clamp(-448, 448)
     assert torch.equal(formulas.e4m3_round(x.double()), x.to(torch.float8_e4m3fn).double())
+
+
+@pytest.mark.parametrize("call,message", [
+    (lambda: build_fp8_gemm(0, 8, 16), "M=0"),
+    (lambda: build_fp8_gemm(1, 12, 16), "divisible by 8"),
+    (lambda: build_fp8_gemm(1, 8, 24), "divisible by 16"),
+    (lambda: build_fp8_gemm(1, 8, 16, out_dtype=f16), "f32 or bf16"),
+    (lambda: build_fp8_grouped_gemm_varlen(1025, 8, 8, 16), "G=1025"),
+    (lambda: build_fp8_grouped_gemm_varlen(2, 0, 8, 16), "M_total=0"),
+])
+def test_fp8_gemm_builders_refuse(call, message):
+    with pytest.raises(AssertionError, match=message):
+        call()
+
+
+@pytest.mark.parametrize("kid,dims,message", [
+    (_ids.K_FP8_GEMM, (1, 12, 16), "divisible by 8"),
+    (_ids.K_FP8_GEMM, (1, 8, 24), "divisible by 16"),
+    (_ids.K_FP8_GEMM, (1, 8), "needs 3 dims"),
+    (_ids.K_FP8_GEMM, (0, 8, 16), "positive"),
+    (_ids.K_FP8_GEMM, (2 ** 31 - 1, 8, 16), "2^31-1"),
+    (_ids.K_FP8_GEMM, (2 ** 30, 2 ** 30, 16), "2^31-1"),
+    (_ids.K_FP8_GROUPED_GEMM, (1025, 8, 8, 16), "G=1025"),
+    (_ids.K_FP8_GROUPED_GEMM, (1024, 8, 2 ** 22, 16), "2^31-1"),
+])
+def test_library_refuses_fp8_gemm(kid, dims, message):
+    rc, text = _create(kid, dims)
+    assert rc == _ids.ERR_BAD_SHAPE and message in text, (rc, text)
+
+
+def test_fp8_gemm_geometry():
+    """Single tokens split K over a cluster; large products fill the SMs with whole tiles."""
+    one = build_fp8_gemm(1, 4096, 4096)
+    assert one.cluster[0] > 1 and one.grid[0] % one.cluster[0] == 0 and one.scratch_bytes == 0
+    big = build_fp8_gemm(8192, 8192, 4096, out_dtype=bf16)
+    assert big.cluster == (1, 1, 1) and 100 < big.grid[0] <= 148 and big.smem <= 227 * 1024
+    grouped = build_fp8_grouped_gemm_varlen(64, 128, 2048, 2064)
+    assert grouped.in_specs[3].shape == (64 * 16, 17) and grouped.in_specs[4].dtype is s32
