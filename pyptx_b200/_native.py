@@ -154,9 +154,11 @@ def build_torch_ext(force: bool = False) -> str:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I" + sysconfig.get_paths()["include"]]
     cmd += ["-I" + i for i in inc if os.path.isdir(i) and "cuda" not in i]
+    cmd += ["-I" + os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(
+        shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))), "include")]      # cuda_runtime_api.h, for the stream type
     libdirs = [d for d in libdirs if os.path.isdir(d) and "cuda" not in d]
     cmd += ["-L" + d for d in libdirs]
-    cmd += ["-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ldl"]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ldl"]
     cmd += ["-Wl,-rpath," + d for d in libdirs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -7,7 +7,17 @@
 // the void*[] of inputs then outputs and makes one call into pb200_launch_raw.  Unlike the
 // reference, the error buffer is per call (no shared static buffer), and inputs are checked
 // for device / contiguity before the call.
+//
+// Launcher is the same launch with everything static bound to the kernel object: one call from
+// Python checks the inputs against the specs, takes the current stream, allocates and launches.
+// A call of ours costs the host about as long as a small kernel runs, so this path decides what a
+// chain of small calls costs (measured on the GPU host: DISPATCH_US_AFTER us a call against DISPATCH_US_BEFORE us with the checks in
+// Python).  It answers None for whatever it does not accept, and the caller takes the checking path,
+// which words the errors.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
 
 #include <dlfcn.h>
 
@@ -66,9 +76,76 @@ std::vector<torch::Tensor> launch_kernel(int64_t handle, int64_t stream,
     return outs;
 }
 
+class Launcher {
+public:
+    Launcher(int64_t handle, std::vector<int64_t> in_dtypes, std::vector<std::vector<int64_t>> in_shapes,
+             std::vector<int64_t> out_dtypes, std::vector<std::vector<int64_t>> out_shapes, int64_t scratch_bytes)
+        : handle_(handle), out_shapes_(std::move(out_shapes)), in_shapes_(std::move(in_shapes)) {
+        for (auto d : in_dtypes) in_dtypes_.push_back(static_cast<c10::ScalarType>(d));
+        for (auto d : out_dtypes) out_dtypes_.push_back(static_cast<c10::ScalarType>(d));
+        n_results_ = out_shapes_.size();
+        if (scratch_bytes > 0) {
+            out_shapes_.push_back({scratch_bytes});
+            out_dtypes_.push_back(c10::ScalarType::Byte);
+        }
+    }
+
+    // One tensor, a tuple of tensors, or None when the inputs are not exactly what the specs say.
+    pybind11::object call(const pybind11::tuple& args) const {
+        const size_t n_in = in_shapes_.size();
+        if (!g_launch_raw || args.size() != n_in || n_in == 0) return pybind11::none();
+        constexpr size_t kMaxBuffers = 32;
+        void* ptrs[kMaxBuffers];
+        if (n_in + out_shapes_.size() > kMaxBuffers) return pybind11::none();
+        c10::Device device(c10::DeviceType::CPU);
+        for (size_t i = 0; i < n_in; ++i) {
+            PyObject* obj = PyTuple_GET_ITEM(args.ptr(), (Py_ssize_t)i);
+            if (!THPVariable_CheckExact(obj)) return pybind11::none();
+            const at::Tensor& t = THPVariable_Unpack(obj);
+            if (!t.is_cuda() || t.layout() != c10::Layout::Strided || t.scalar_type() != in_dtypes_[i] ||
+                t.sizes() != c10::IntArrayRef(in_shapes_[i]) || !t.is_contiguous())
+                return pybind11::none();
+            if (i == 0) device = t.device();
+            else if (t.device() != device) return pybind11::none();
+            ptrs[i] = t.data_ptr();
+        }
+        if (c10::cuda::current_device() != device.index()) return pybind11::none();
+        const uint64_t stream = (uint64_t)(uintptr_t)c10::cuda::getCurrentCUDAStream(device.index()).stream();
+        std::vector<at::Tensor> outs;
+        outs.reserve(out_shapes_.size());
+        for (size_t i = 0; i < out_shapes_.size(); ++i) {
+            outs.push_back(torch::empty(out_shapes_[i], torch::TensorOptions().dtype(out_dtypes_[i]).device(device)));
+            ptrs[n_in + i] = outs.back().data_ptr();
+        }
+        char err[128] = {0};
+        int rc;
+        {
+            pybind11::gil_scoped_release nogil;
+            rc = g_launch_raw(handle_, stream, ptrs, n_in + outs.size(), err);
+        }
+        if (rc != 0)
+            throw std::runtime_error("pyptx_b200: pb200_launch_raw failed (code " + std::to_string(rc) + "): " + err);
+        if (n_results_ == 1) return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(outs[0]));
+        pybind11::tuple res(n_results_);
+        for (size_t i = 0; i < n_results_; ++i)
+            PyTuple_SET_ITEM(res.ptr(), (Py_ssize_t)i, THPVariable_Wrap(outs[i]));
+        return res;
+    }
+
+private:
+    int64_t handle_;
+    size_t n_results_ = 0;
+    std::vector<std::vector<int64_t>> out_shapes_, in_shapes_;
+    std::vector<c10::ScalarType> in_dtypes_, out_dtypes_;
+};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("load_shim", &load_shim, "dlopen the C-ABI library");
     m.def("launch_kernel", &launch_kernel, "allocate outputs and launch a registered kernel");
+    pybind11::class_<Launcher>(m, "Launcher")
+        .def(pybind11::init<int64_t, std::vector<int64_t>, std::vector<std::vector<int64_t>>, std::vector<int64_t>,
+                            std::vector<std::vector<int64_t>>, int64_t>())
+        .def("call", &Launcher::call, "check, allocate and launch; None when the inputs need the checking path");
 }

@@ -12,7 +12,7 @@ from __future__ import annotations
 import sys
 from typing import Any, Sequence
 
-from . import _native
+from . import _native, torch_support
 from .specs import Tile, unify_envs
 
 
@@ -51,7 +51,6 @@ class NativeKernel:
         # call, so it is registered here whenever torch is already imported.
         self._op = None
         if "torch" in sys.modules:
-            from . import torch_support
             self._op = torch_support.get_or_register_torch_op(self)
 
     # -- attribute surface of the reference's Kernel -------------------------
@@ -114,8 +113,12 @@ class NativeKernel:
         return [spec.resolve_shape(env or {}) for spec in self._out_specs]
 
     def __call__(self, *args: Any) -> Any:
-        from . import torch_support
-
+        if not torch_support.is_compiling():
+            launcher = self._launcher
+            if launcher is not None and launcher.ext is not None and launcher.fast is not None:
+                out = launcher.fast(args)
+                if out is not None:
+                    return out
         inputs = args[: len(self._in_specs)]
         if len(inputs) != len(self._in_specs):
             raise TypeError(

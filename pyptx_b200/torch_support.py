@@ -36,6 +36,11 @@ def _torch():
     return _TORCH
 
 
+def is_compiling() -> bool:
+    """Whether Dynamo is tracing the caller (calls then go through the registered op)."""
+    return _torch().compiler.is_compiling()
+
+
 def is_torch_tensor(obj: Any) -> bool:
     try:
         return isinstance(obj, _torch().Tensor)
@@ -110,6 +115,13 @@ class _Launcher:
                  torch.float8_e4m3fn: 24}
         self.out_dtype_codes = [codes[d] for d in self.out_dtypes]
         self.handle_int = int(kernel.handle)
+        # One call from Python does checks, allocation and launch; only for fully static specs.
+        self.fast = None
+        if self.ext is not None and self.static_out_shapes is not None and None not in self.in_shapes \
+                and all(d in codes for d in self.in_dtypes):
+            self.fast = self.ext.Launcher(
+                self.handle_int, [codes[d] for d in self.in_dtypes], [list(s) for s in self.in_shapes],
+                self.out_dtype_codes, [list(s) for s in self.static_out_shapes], self.scratch_bytes).call
 
 
     def call_buffers(self):
@@ -231,8 +243,7 @@ def get_or_register_torch_op(kernel):
 def call_kernel(kernel, inputs: Sequence[Any]):
     """Dispatch used by ``NativeKernel.__call__``: the registered op while Dynamo
     is tracing, the direct launch otherwise; one output -> tensor, several -> tuple."""
-    torch = _torch()
-    if torch.compiler.is_compiling():
+    if is_compiling():
         op = kernel._op
         if op is None:
             raise RuntimeError(
