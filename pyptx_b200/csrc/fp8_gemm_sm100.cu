@@ -33,16 +33,24 @@ using namespace ptx;
 
 constexpr int BM = 128;
 constexpr int BK = 128;                      // one scale block of K = one 128-byte swizzle row of e4m3
-constexpr int kThreads = 384;                // 12 warps: 4 of control, 8 of epilogue
-constexpr int kEpiWarps = 8;
 constexpr int kSmallRows = 32;               // row box of A for tiles with few rows
-constexpr int kRing = 192 * 1024;            // operand ring
-constexpr int kChunkBytes = 64;              // bytes of a row that a warp stages at a time
-constexpr int kStageBytes = 32 * kChunkBytes;
+constexpr int kStages = 4;
+constexpr int kStage = 32 * 1024;            // 128 x 128 of A and 128 x 128 of B_T
+constexpr int kRing = kStages * kStage;
+constexpr int kBoxBytes = 32 * 128;          // a warp's store box: 32 rows of 128 bytes
+constexpr int kBoxes = 2;                    // of them in flight for each epilogue warp
+constexpr int kEpiWarps = 8;
+constexpr int kOutBytes = kEpiWarps * kBoxes * kBoxBytes;
+constexpr int kThreads = 128 + 32 * kEpiWarps;       // 4 warps of control
+constexpr int kAccCols = 128;                // TMEM columns of an accumulator
+constexpr int kAccs = 4;                     // accumulators: all of TMEM
 constexpr int kMaxExperts = 1024;
 constexpr int kTableBytes = 2 * (kMaxExperts + 1) * 4 + 120;      // sanitised offsets and tile prefix, padded to 128
 constexpr int kBarBytes = 1024;
-constexpr int kSmemTotal = 1024 + kRing + kEpiWarps * kStageBytes + kTableBytes + kBarBytes;
+constexpr int kGroup = 8;                    // scale blocks whose scales are fetched together (one 32-byte sector of a row)
+constexpr int kScaleWords = kGroup * BM + 2 * kGroup;             // of a group: 128 rows', two column blocks'
+constexpr int kScaleBytes = (2 * kScaleWords * 4 + 127) / 128 * 128;
+constexpr int kSmemTotal = 1024 + kRing + kOutBytes + kTableBytes + kScaleBytes + kBarBytes;
 static_assert(kSmemTotal <= 227 * 1024, "shared memory");
 constexpr int kMaxSplit = 8;
 // Registers of the 256-column form, whose epilogue threads hold 128 sums: the launch has 384 x 168;
@@ -55,12 +63,26 @@ constexpr int kPartPitch = 128 + 4;          // f32 row pitch of a split's parti
 constexpr uint32_t make_idesc_e4m3(int m, int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+template <int CTA_GROUP>
 __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
                                            uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %6, 0;\n"
-                 "mov.b64 da, {%1, %2};\nmov.b64 db, {%3, %4};\n"
-                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n}"
-                 :: "r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
+    if (CTA_GROUP == 1)
+        asm volatile("{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %6, 0;\n"
+                     "mov.b64 da, {%1, %2};\nmov.b64 db, {%3, %4};\n"
+                     "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n}"
+                     :: "r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\n.reg .b64 da, db;\nsetp.ne.b32 p, %6, 0;\n"
+                     "mov.b64 da, {%1, %2};\nmov.b64 db, {%3, %4};\n"
+                     "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p;\n}"
+                     :: "r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Arrival at a barrier of the pair's leader with release at CTA scope: what it publishes is the end of
+// TMEM reads (ordered by tcgen05.fence), no memory writes, and the cluster-scope release of
+// mbar_arrive_cluster costs the warp about 1400 clocks on each block.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(bar_cluster_addr) : "memory");
 }
 
 struct Shape {
@@ -79,38 +101,46 @@ struct TilePos {
     int row0, row_end, col0, expert;
 };
 
+// BN = 256: a pair of CTAs works on 256 x 256 tiles (cta_group::2).  BN = 128: one CTA, 128 x 128 tiles.
 template <int BN, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a_small,
-                const __grid_constant__ CUtensorMap tmap_b, const float* __restrict__ a_scale,
+                const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_d, const float* __restrict__ a_scale,
                 const float* __restrict__ b_scale, const int* __restrict__ offsets, OutT* __restrict__ out, Shape shape,
                 int* status, int kernel_id) {
+    constexpr int CTA_GROUP = BN / 128;
+    constexpr int kHalves = BN / kAccCols;                    // accumulators of a block: one for each 128 columns
     constexpr int kABytes = BM * BK;
-    constexpr int kStage = kABytes + BN * BK;
-    constexpr int kStages = kRing / kStage;
-    constexpr int kAccs = 512 / BN > 4 ? 4 : 512 / BN;        // accumulators in TMEM
-    constexpr uint32_t kTmemCols = kAccs * BN;
-    constexpr uint32_t kIdesc = make_idesc_e4m3(BM, BN);
-    constexpr int kCols = BN / 2;                             // columns of an epilogue warp
+    constexpr int kBRows = kAccCols / CTA_GROUP;              // rows of B_T this CTA loads for an accumulator
+    static_assert(kABytes + kHalves * kBRows * BK == kStage, "ring stage");
+    constexpr int kTileRows = BM * CTA_GROUP;
+    constexpr uint32_t kTmemCols = kAccs * kAccCols;
+    constexpr uint32_t kIdesc = make_idesc_e4m3(kTileRows, kAccCols);
+    constexpr int kCols = BN / 2;                             // columns of an epilogue warp: f32 sums of a thread
+    constexpr int kColBlocks = BN / BK;                       // scale blocks of a tile's columns
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t s_ring = smem_base;
-    const uint32_t s_epi = s_ring + kRing;
-    const uint32_t s_bar = s_epi + kEpiWarps * kStageBytes + kTableBytes;
-    int* seg = reinterpret_cast<int*>(smem_gen + kRing + kEpiWarps * kStageBytes);     // [experts+1] row offsets
-    int* seg_tile = seg + kMaxExperts + 1;                                             // [experts+1] M-tiles before
+    const uint32_t s_bar = s_ring + kRing + kOutBytes + kTableBytes + kScaleBytes;
+    int* seg = reinterpret_cast<int*>(smem_gen + kRing + kOutBytes);      // [experts+1] row offsets
+    int* seg_tile = seg + kMaxExperts + 1;                    // [experts+1] M-tiles before
+    const uint32_t s_scales = s_ring + kRing + kOutBytes + kTableBytes;      // 2 x ([kGroup][BM] of A, [kColBlocks][kGroup] of B)
+    const float* scales = reinterpret_cast<const float*>(smem_gen + (s_scales - smem_base));
     const uint32_t bar_full = s_bar, bar_empty = bar_full + 8 * kStages;
     const uint32_t bar_tfull = bar_empty + 8 * kStages, bar_tempty = bar_tfull + 8 * kAccs;
-    const uint32_t s_tmem_slot = bar_tempty + 8 * kAccs, s_abort = s_tmem_slot + 8;
+    const uint32_t bar_sfull = bar_tempty + 8 * kAccs, bar_sempty = bar_sfull + 16;
+    const uint32_t s_tmem_slot = bar_sempty + 16, s_abort = s_tmem_slot + 8;
     volatile uint32_t* tmem_slot_gen = (volatile uint32_t*)(smem_gen + (s_tmem_slot - smem_base));
     volatile int* abort_gen = (volatile int*)(smem_gen + (s_abort - smem_base));
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
+    const int lane = threadIdx.x & 31;
+    const uint32_t pair_rank = CTA_GROUP == 2 ? cluster_ctarank() : 0u;
     const int split = BN == 128 ? shape.split : 1;            // only the 128-column form splits K
     const int split_rank = split > 1 ? (int)cluster_ctarank() : 0;
-    const int unit = (int)blockIdx.x / split, n_units = (int)gridDim.x / split;
+    const int unit = (int)blockIdx.x / (split * CTA_GROUP), n_units = (int)gridDim.x / (split * CTA_GROUP);
     // this CTA's scale blocks of K
     const int kb0 = (int)((long long)shape.blocks * split_rank / split);
     const int kb1 = (int)((long long)shape.blocks * (split_rank + 1) / split);
@@ -124,16 +154,21 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
         for (int b = 0; b < kAccs; ++b) {
             mbar_init(bar_tfull + 8 * b, 1);
-            mbar_init(bar_tempty + 8 * b, kEpiWarps);
+            mbar_init(bar_tempty + 8 * b, kEpiWarps / kHalves * CTA_GROUP);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(bar_sfull + 8 * b, 32);
+            mbar_init(bar_sempty + 8 * b, kEpiWarps);
         }
         fence_mbarrier_init();
         fence_proxy_async_smem();
         prefetch_tmap(&tmap_a);
         prefetch_tmap(&tmap_b);
+        prefetch_tmap(&tmap_d);
     }
     if (warp == 1) {
-        tmem_alloc<1>(s_tmem_slot, kTmemCols);
-        tmem_relinquish<1>();
+        tmem_alloc<CTA_GROUP>(s_tmem_slot, kTmemCols);
+        tmem_relinquish<CTA_GROUP>();
     }
     pdl_launch_dependents();
     pdl_wait();
@@ -155,7 +190,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             end = max(end, run_max);
             int start = __shfl_up_sync(0xffffffffu, end, 1);
             if (lane == 0) start = run_max;
-            int tiles = (end - start + BM - 1) / BM;
+            int tiles = (end - start + kTileRows - 1) / kTileRows;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, tiles, o);
@@ -168,7 +203,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
     }
     tc_fence_before_sync();
-    __syncthreads();
+    if (CTA_GROUP == 2) cluster_sync_all(); else __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot_gen;
     const int n_tiles = (shape.experts > 0 ? seg_tile[shape.experts] : shape.tiles_m) * shape.tiles_n;
@@ -184,7 +219,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const int r = t - seg_tile[lo] * shape.tiles_n, width = seg_tile[lo + 1] - seg_tile[lo];
             const int tn = r / width;                // an expert's M-tiles share a block of weights: M fastest
             p.expert = lo;
-            p.row0 = seg[lo] + (r - tn * width) * BM;
+            p.row0 = seg[lo] + (r - tn * width) * kTileRows;
             p.row_end = seg[lo + 1];
             p.col0 = tn * BN;
         } else {
@@ -193,7 +228,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const int m0 = b * shape.band, width = min(shape.band, shape.tiles_m - m0);
             const int tn = r / width;
             p.expert = 0;
-            p.row0 = (m0 + r - tn * width) * BM;
+            p.row0 = (m0 + r - tn * width) * kTileRows;
             p.row_end = shape.m;
             p.col0 = tn * BN;
         }
@@ -205,93 +240,169 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         if (warp == 0 && lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
+            const uint32_t full_leader = CTA_GROUP == 2 ? map_to_cta(bar_full, 0) : bar_full;
             bool ok = true;
             for (int t = unit; t < n_tiles && ok; t += n_units) {
                 const TilePos p = tile_pos(t);
-                const bool small = p.row_end - p.row0 <= kSmallRows;
-                const int row_b = p.expert * shape.n + p.col0;
+                const int row_a = p.row0 + (int)pair_rank * BM;
+                const bool small = p.row_end - row_a <= kSmallRows;
+                const int row_b = p.expert * shape.n + p.col0 + (int)pair_rank * kBRows;      // of the first half
+                // bytes of this CTA's loads, and for the leader of a pair its peer's too
+                uint32_t tx = 0;
+#pragma unroll
+                for (int c = 0; c < CTA_GROUP; ++c)
+                    tx += (uint32_t)((p.row_end - p.row0 - c * BM <= kSmallRows ? kSmallRows * BK : kABytes) + kHalves * kBRows * BK);
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, ctx, 1))) break;
                     const uint32_t dst = s_ring + stage * kStage, bar = bar_full + 8 * stage;
-                    mbar_arrive_expect_tx(bar, (uint32_t)((small ? kSmallRows * BK : kABytes) + BN * BK));
-                    tma_load_2d(dst + kABytes, &tmap_b, bar, kb * BK, row_b);
-                    tma_load_2d(dst, small ? &tmap_a_small : &tmap_a, bar, kb * BK, p.row0);
+                    if (CTA_GROUP == 1) {
+                        mbar_arrive_expect_tx(bar, tx);
+                        tma_load_2d(dst + kABytes, &tmap_b, bar, kb * BK, row_b);
+                        tma_load_2d(dst, small ? &tmap_a_small : &tmap_a, bar, kb * BK, row_a);
+                    } else {
+                        if (pair_rank == 0) mbar_arrive_expect_tx(bar, tx);
+#pragma unroll
+                        for (int h = 0; h < kHalves; ++h)
+                            tma_load_2d_pair(dst + kABytes + h * kBRows * BK, &tmap_b, full_leader + 8 * stage, kb * BK, row_b + h * kAccCols);
+                        tma_load_2d_pair(dst, small ? &tmap_a_small : &tmap_a, full_leader + 8 * stage, kb * BK, row_a);
+                    }
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
             }
         }
-        if (warp == 1 && lane == 0) {
+        if (warp == 1 && pair_rank == 0 && unit < n_tiles) {
+            // The whole warp runs the loop and one elected lane issues (see elect_one): with descriptors in
+            // uniform registers an MMA issues in a few clocks, from a lane's own registers in about 60, which is
+            // as long as it executes, so that every wait would be a hole in the tensor pipe.
+            const int total = ((n_tiles - unit - 1) / n_units + 1) * (kb1 - kb0);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             const uint64_t da0 = make_desc_kmajor_sw128(s_ring), db0 = make_desc_kmajor_sw128(s_ring + kABytes);
             const uint32_t a_hi = (uint32_t)(da0 >> 32), b_hi = (uint32_t)(db0 >> 32);
+            const bool leader = elect_one();
             bool ok = true;
-            for (int t = unit; t < n_tiles && ok; t += n_units) {
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!(ok = mbar_wait(bar_tempty + 8 * acc, acc_phase ^ 1u, ctx, 2))) break;
-                    if (!(ok = mbar_wait(bar_full + 8 * stage, phase, ctx, 3))) break;
-                    tc_fence_after_sync();
-                    const uint32_t a_lo = (uint32_t)da0 + (uint32_t)(stage * (kStage >> 4));
-                    const uint32_t b_lo = (uint32_t)db0 + (uint32_t)(stage * (kStage >> 4));
-                    const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+            for (int i = 0; i < total && ok; ++i) {
+                ok = mbar_wait(bar_full + 8 * stage, phase, ctx, 3);
+                const uint32_t a_lo = (uint32_t)da0 + (uint32_t)(stage * (kStage >> 4));
+                const uint32_t b_lo = (uint32_t)db0 + (uint32_t)(stage * (kStage >> 4));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)      // 32 e4m3 along K = 32 bytes = +2 in the encoded address
-                        umma_f8_ss(d, a_lo + 2 * i, a_hi, b_lo + 2 * i, b_hi, kIdesc, i != 0 ? 1u : 0u);
-                    umma_commit<1>(bar_empty + 8 * stage);
-                    umma_commit<1>(bar_tfull + 8 * acc);
-                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                for (int h = 0; h < kHalves; ++h) {
+                    if (ok) ok = mbar_wait(bar_tempty + 8 * acc, acc_phase ^ 1u, ctx, 2);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint32_t d = tmem_base + (uint32_t)(acc * kAccCols);
+                    if (leader) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)      // 32 e4m3 along K = 32 bytes = +2 in the encoded address
+                            umma_f8_ss<CTA_GROUP>(d, a_lo + 2 * j, a_hi, b_lo + (uint32_t)(h * (kBRows * BK >> 4)) + 2 * j, b_hi, kIdesc,
+                                                  j != 0 ? 1u : 0u);
+                        if (CTA_GROUP == 2) umma_commit_pair(bar_tfull + 8 * acc); else umma_commit<1>(bar_tfull + 8 * acc);
+                        if (h == kHalves - 1) {
+                            if (CTA_GROUP == 2) umma_commit_pair(bar_empty + 8 * stage); else umma_commit<1>(bar_empty + 8 * stage);
+                        }
+                    }
+                    __syncwarp();
                     if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
                 }
+                if (++stage == kStages) { stage = 0; phase ^= 1u; }
             }
+        }
+        if (warp == 3) {
+            // Scales: this warp copies a group of blocks ahead into shared memory (four rows a lane), so that
+            // no epilogue warp waits for global memory.
+            int buf = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = unit; t < n_tiles && ok; t += n_units) {
+                const TilePos p = tile_pos(t);
+                const int row0 = p.row0 + (int)pair_rank * BM + lane;
+                // lane c * kGroup + i copies block i's scale of column block c
+                const int cb = lane / kGroup, ib = lane % kGroup;
+                const bool b_there = cb < kColBlocks && p.col0 + cb * BK < shape.n;
+                const float* sb = b_scale + ((long long)p.expert * shape.n_blocks + p.col0 / BK + (b_there ? cb : 0)) * shape.blocks;
+                for (int kb = kb0; kb < kb1; kb += kGroup) {
+                    ok = mbar_wait(bar_sempty + 8 * buf, phase ^ 1u, ctx, 5);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const uint32_t dst = s_scales + (uint32_t)(buf * kScaleWords + lane) * 4u;
+#pragma unroll 1
+                    for (int j = 0; j < 4; ++j) {
+                        const bool there = row0 + 32 * j < p.row_end;
+                        const float* sa = a_scale + (there ? (long long)(row0 + 32 * j) * shape.blocks : 0ll);
+#pragma unroll
+                        for (int i = 0; i < kGroup; ++i)      // blocks past the end: any word of the row, never used
+                            cp_async_4(dst + (uint32_t)(i * BM + 32 * j) * 4u, sa + min(kb + i, kb1 - 1), there);
+                    }
+                    if (lane < 2 * kGroup) cp_async_4(dst + kGroup * BM * 4u, sb + min(kb + ib, kb1 - 1), b_there);
+                    cp_async_arrive(bar_sfull + 8 * buf);
+                    if (++buf == 2) { buf = 0; phase ^= 1u; }
+                }
+            }
+            cp_async_wait_all();
         }
     } else {
         if (BN == 256) reg_alloc<kEpilogueRegs>();
-        const int q = warp & 3, half = (warp - 4) >> 2;
-        const uint32_t stage_buf = s_epi + (uint32_t)(warp - 4) * kStageBytes;
-        int acc = 0;
-        uint32_t acc_phase = 0;
+        const int q = warp & 3, group = (warp - 4) >> 2;
+        const uint32_t box = s_ring + kRing + (uint32_t)(warp - 4) * (kBoxes * kBoxBytes);
+        const uint32_t tempty_leader = CTA_GROUP == 2 ? map_to_cta(bar_tempty, 0) : bar_tempty;
+        constexpr int kAccStep = kHalves;            // this warp's accumulators: those of its half
+        const int acc0 = kHalves == 2 ? group : 0, col_in_acc = kHalves == 2 ? 0 : group * kCols;
+        int acc = acc0, sbuf = 0;
+        uint32_t acc_phase = 0, sphase = 0;
         bool ok = true;
         for (int t = unit; t < n_tiles && ok; t += n_units) {
             const TilePos p = tile_pos(t);
-            const int row = p.row0 + q * 32 + lane;                  // this thread's row
-            const int col = p.col0 + half * kCols;                   // this warp's first column
-            const float* sa = row < p.row_end ? a_scale + (long long)row * shape.blocks : nullptr;
-            const float* sb = col < shape.n ? b_scale + ((long long)p.expert * shape.n_blocks + col / BK) * shape.blocks : nullptr;
+            const int row = p.row0 + (int)pair_rank * BM + q * 32 + lane;      // this thread's row
+            const int col = p.col0 + group * kCols;                   // this warp's first column
             float sum[kCols];
 #pragma unroll
             for (int i = 0; i < kCols; ++i) sum[i] = 0.0f;
-            float s_next = sa && sb && kb0 < kb1 ? __ldg(sa + kb0) * __ldg(sb + kb0) : 0.0f;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const float s = s_next;
-                ok = mbar_wait(bar_tfull + 8 * acc, acc_phase, ctx, 4);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after_sync();
-                if (sa && sb && kb + 1 < kb1) s_next = __ldg(sa + kb + 1) * __ldg(sb + kb + 1);
-                const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + half * kCols);
+            for (int kb = kb0; kb < kb1 && ok; kb += kGroup) {
+                ok = mbar_wait(bar_sfull + 8 * sbuf, sphase, ctx, 6);
+                const float* sa = scales + sbuf * kScaleWords + q * 32 + lane;
+                const float* sb = scales + sbuf * kScaleWords + kGroup * BM + group * kCols / BK * kGroup;
+                const int n_blocks = min(kGroup, kb1 - kb);
+                for (int i = 0; i < n_blocks; ++i) {
+                    if (ok) ok = mbar_wait(bar_tfull + 8 * acc, acc_phase, ctx, 4);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const float s = sa[i * BM] * sb[i];
+                    const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kAccCols + col_in_acc);
+                    constexpr int kChunks = kCols / 32;
+                    uint32_t v[2][32];                       // the next 32 columns arrive under the FMAs
+                    tmem_ld_32x32b_x32(t_row, v[0]);
 #pragma unroll
-                for (int c = 0; c < kCols / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld_32x32b_x32(t_row + c * 32, v);
-                    tmem_ld_wait();
-                    reg_fence(v);
-                    if (c == kCols / 32 - 1) {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
+                    for (int c = 0; c < kChunks; ++c) {
+                        tmem_ld_wait();
+                        reg_fence(v[c & 1]);
+                        if (c + 1 < kChunks) {
+                            tmem_ld_32x32b_x32(t_row + (c + 1) * 32, v[(c + 1) & 1]);
+                        } else {
+                            tc_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (CTA_GROUP == 2) mbar_arrive_remote(tempty_leader + 8 * acc);
+                                else mbar_arrive(bar_tempty + 8 * acc);
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2)
+                            fma2v(sum[c * 32 + j], sum[c * 32 + j + 1], __uint_as_float(v[c & 1][j]), __uint_as_float(v[c & 1][j + 1]),
+                                  s, s, sum[c * 32 + j], sum[c * 32 + j + 1]);
                     }
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        fma2v(sum[c * 32 + i], sum[c * 32 + i + 1], __uint_as_float(v[i]), __uint_as_float(v[i + 1]), s, s,
-                              sum[c * 32 + i], sum[c * 32 + i + 1]);
+                    if ((acc += kAccStep) >= kAccs) { acc = acc0; acc_phase ^= 1u; }
                 }
-                if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_sempty + 8 * sbuf);
+                if (++sbuf == 2) { sbuf = 0; sphase ^= 1u; }
             }
             if (!ok) break;
             if (split > 1) {
                 // One tile a cluster: the ring is drained (every MMA that read it has been waited for
                 // through its accumulator), so the partial tile goes there.
-                float* part = reinterpret_cast<float*>(smem_gen) + (q * 32 + lane) * kPartPitch + half * kCols;
+                float* part = reinterpret_cast<float*>(smem_gen) + (q * 32 + lane) * kPartPitch + group * kCols;
                 if (row < p.row_end) {
 #pragma unroll
                     for (int i = 0; i < kCols; i += 4)
@@ -299,37 +410,45 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 }
                 break;
             }
-            constexpr int kChunkCols = kChunkBytes / (int)sizeof(OutT);
+            constexpr int kBoxCols = 128 / (int)sizeof(OutT);
+            const int row_w = p.row0 + (int)pair_rank * BM + q * 32;      // first row of this warp
+            // TMA clips a box at the matrix's edges, but not at the end of an expert's rows.
+            const bool whole = shape.experts == 0 || row_w + 32 <= p.row_end;
 #pragma unroll
-            for (int c = 0; c < kCols / kChunkCols; ++c) {
-                uint32_t w[16];
+            for (int c = 0; c < kCols / kBoxCols; ++c) {
+                uint32_t w[32];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < 32; ++i) {
                     if (sizeof(OutT) == 4) {
-                        w[i] = __float_as_uint(sum[c * kChunkCols + i]);
+                        w[i] = __float_as_uint(sum[c * kBoxCols + i]);
                     } else {
-                        __nv_bfloat162 b2 = __floats2bfloat162_rn(sum[c * kChunkCols + 2 * i], sum[c * kChunkCols + 2 * i + 1]);
+                        __nv_bfloat162 b2 = __floats2bfloat162_rn(sum[(c * kBoxCols + 2 * i) % kCols], sum[(c * kBoxCols + 2 * i + 1) % kCols]);
                         w[i] = *reinterpret_cast<uint32_t*>(&b2);
                     }
                 }
-                __syncwarp();
+                if (whole) {
+                    const uint32_t buf = box + (uint32_t)(c % kBoxes) * kBoxBytes;
+                    if (lane == 0) tma_store_wait_read<kBoxes - 1>();      // the store that last read this buffer
+                    __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    st_shared_v4(stage_buf + (uint32_t)(lane * kChunkBytes + ((j ^ ((lane >> 1) & 3)) << 4)),
-                                 w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-                __syncwarp();
-                const int j = lane & 3, c_out = col + c * kChunkCols + j * (16 / (int)sizeof(OutT));
+                    for (int j = 0; j < 8; ++j)
+                        st_shared_v4(buf + (uint32_t)(lane * 128 + ((j ^ (lane & 7)) << 4)), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (row_w < p.row_end && col + c * kBoxCols < shape.n) tma_store_2d(&tmap_d, buf, col + c * kBoxCols, row_w);
+                        tma_store_commit();
+                    }
+                } else if (row < p.row_end) {
+                    OutT* dst = out + (long long)row * shape.n + col + c * kBoxCols;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = i * 8 + (lane >> 2), r_out = p.row0 + q * 32 + r;
-                    uint32_t x0, x1, x2, x3;
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x0), "=r"(x1), "=r"(x2), "=r"(x3)
-                                 : "r"(stage_buf + (uint32_t)(r * kChunkBytes + ((j ^ ((r >> 1) & 3)) << 4))) : "memory");
-                    if (r_out < p.row_end && c_out < shape.n)
-                        *reinterpret_cast<uint4*>(out + (long long)r_out * shape.n + c_out) = make_uint4(x0, x1, x2, x3);
+                    for (int j = 0; j < 8; ++j)
+                        if (col + c * kBoxCols + j * (16 / (int)sizeof(OutT)) < shape.n)
+                            reinterpret_cast<uint4*>(dst)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                 }
             }
         }
+        if (lane == 0) tma_store_wait_read<0>();      // shared memory must outlive the stores' reads
     }
 
     __syncwarp();
@@ -369,13 +488,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             }
         }
         cluster_sync_all();
+    } else if (CTA_GROUP == 2) {
+        cluster_sync_all();
     } else {
         __syncthreads();
     }
     if (warp == 1) {
         __syncwarp();
         tc_fence_after_sync();
-        tmem_dealloc<1>(tmem_base, kTmemCols);
+        tmem_dealloc<CTA_GROUP>(tmem_base, kTmemCols);
     }
 }
 
@@ -387,6 +508,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Plan {
     int64_t experts, m, n, k, tiles;
     int bn, split;
+    int cta_group() const { return bn / 128; }
 };
 
 // Tile width and split of K.
@@ -405,11 +527,11 @@ Plan make_plan(const Record& r) {
     if (grouped) {
         p.bn = p.n > 128 ? 256 : 128;
         // every expert may end in a partial tile
-        p.tiles = (mt + p.experts) * ceil_div(p.n, p.bn);
+        p.tiles = (ceil_div(p.m, BM * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);
         return p;
     }
     p.bn = mt * ceil_div(p.n, 256) >= sms ? 256 : 128;
-    p.tiles = mt * ceil_div(p.n, p.bn);
+    p.tiles = ceil_div(p.m, BM * p.cta_group()) * ceil_div(p.n, p.bn);
     if (p.bn == 128) {
         const int64_t blocks = ceil_div(p.k, BK);
         while (p.split < kMaxSplit && p.tiles * p.split * 2 <= sms && blocks >= 4 * p.split) p.split *= 2;
@@ -417,8 +539,15 @@ Plan make_plan(const Record& r) {
     return p;
 }
 
+// CTAs of a launch: whole clusters, one for each tile or as many as the SMs hold.
+int64_t grid_of(const Plan& p) {
+    const int64_t cluster = p.split * p.cta_group(), most = p.split > 1 ? p.tiles : sm_count() / p.cta_group();
+    return (p.tiles < most ? p.tiles : most) * cluster;
+}
+
 template <int BN, typename OutT>
 int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** ptrs, char* err) {
+    constexpr int CTA_GROUP = BN / 128;
     auto kernel = fp8_gemm_kernel<BN, OutT>;
     static std::atomic<uint64_t> attr_set{0};   // bit per device
     int dev = 0;
@@ -437,20 +566,27 @@ int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** p
     CUtensorMap ta, ta_small, tb;
     if (int rc = map(&ta, ptrs[0], p.m, BM)) return rc;
     if (int rc = map(&ta_small, ptrs[0], p.m, kSmallRows)) return rc;
-    if (int rc = map(&tb, ptrs[2], p.n * (p.experts ? p.experts : 1), BN)) return rc;
+    if (int rc = map(&tb, ptrs[2], p.n * (p.experts ? p.experts : 1), kAccCols / CTA_GROUP)) return rc;
+    CUtensorMap td;
+    {
+        uint64_t dims[2] = {(uint64_t)p.n, (uint64_t)p.m};
+        uint64_t str[1] = {(uint64_t)p.n * sizeof(OutT)};
+        uint32_t box[2] = {128 / sizeof(OutT), 32};
+        if (int rc = make_tensor_map(&td, sizeof(OutT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                                     ptrs[p.experts ? 5 : 4], dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B, err)) return rc;
+    }
     Shape s;
     s.m = (int)p.m;
     s.n = (int)p.n;
     s.blocks = (int)ceil_div(p.k, BK);
-    s.tiles_m = (int)ceil_div(p.m, BM);
+    s.tiles_m = (int)ceil_div(p.m, BM * CTA_GROUP);
     s.tiles_n = (int)ceil_div(p.n, BN);
     s.band = s.tiles_m < 16 ? s.tiles_m : 16;
     s.experts = (int)p.experts;
     s.n_blocks = (int)ceil_div(p.n, BK);
     s.split = p.split;
-    const int64_t sms = sm_count();
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(p.split > 1 ? p.tiles * p.split : p.tiles < sms ? p.tiles : sms));
+    cfg.gridDim = dim3((unsigned)grid_of(p));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmemTotal;
     cfg.stream = stream;
@@ -458,18 +594,18 @@ int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** p
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)p.split;
+    attr[1].val.clusterDim.x = (unsigned)(p.split * CTA_GROUP);
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = p.split > 1 ? 2 : 1;
+    cfg.numAttrs = p.split * CTA_GROUP > 1 ? 2 : 1;
     const bool grouped = p.experts > 0;
     const int* offsets = grouped ? (const int*)ptrs[4] : nullptr;
     OutT* out = (OutT*)ptrs[grouped ? 5 : 4];
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ta, ta_small, tb, (const float*)ptrs[1], (const float*)ptrs[3], offsets, out, s,
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ta, ta_small, tb, td, (const float*)ptrs[1], (const float*)ptrs[3], offsets, out, s,
                                        device_status_ptr(), (int)r.kernel_id);
     if (e != cudaSuccess) {
-        set_err(err, "fp8 gemm launch failed (BN=%d split=%d): %s", BN, p.split, cudaGetErrorString(e));
-        return p.split > 1 ? PB200_ERR_CLUSTER : PB200_ERR_LAUNCH;
+        set_err(err, "fp8 gemm launch failed (BN=%d cta_group=%d split=%d): %s", BN, CTA_GROUP, p.split, cudaGetErrorString(e));
+        return p.split * CTA_GROUP > 1 ? PB200_ERR_CLUSTER : PB200_ERR_LAUNCH;
     }
     return PB200_OK;
 }
@@ -489,18 +625,17 @@ int plan_fp8_gemm(Record& r, char* err) {
     if (p.n % 8 != 0) { set_err(err, "N=%lld must be divisible by 8", (long long)p.n); return PB200_ERR_BAD_SHAPE; }
     if (p.k % 16 != 0) { set_err(err, "K=%lld must be divisible by 16", (long long)p.k); return PB200_ERR_BAD_SHAPE; }
     // row coordinates of a tile run up to a tile past the last row
-    if (p.m + BM > 0x7fffffffLL || (grouped ? p.experts : 1) * p.n + 256 > 0x7fffffffLL || p.k + BK > 0x7fffffffLL ||
+    if (p.m + 2 * BM > 0x7fffffffLL || (grouped ? p.experts : 1) * p.n + 256 > 0x7fffffffLL || p.k + BK > 0x7fffffffLL ||
         p.tiles > 0x3fffffffLL) {
         set_err(err, "extent exceeds 2^31-1");
         return PB200_ERR_BAD_SHAPE;
     }
     pb200_geometry& g = r.geom;
-    const int64_t sms = sm_count();
-    g.grid[0] = (uint32_t)(p.split > 1 ? p.tiles * p.split : p.tiles < sms ? p.tiles : sms);
+    g.grid[0] = (uint32_t)grid_of(p);
     g.grid[1] = g.grid[2] = 1;
     g.block[0] = kThreads;
     g.block[1] = g.block[2] = 1;
-    g.cluster[0] = (uint32_t)p.split;
+    g.cluster[0] = (uint32_t)(p.split * p.cta_group());
     g.cluster[1] = g.cluster[2] = 1;
     g.smem_bytes = kSmemTotal;
     g.n_inputs = grouped ? 5 : 4;

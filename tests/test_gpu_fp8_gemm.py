@@ -141,7 +141,7 @@ def _grouped(counts, N, K, kind, capacity=None, first=0):
 @pytest.mark.parametrize("counts,N,K", [
     ([1], 8, 16), ([0, 1, 0], 128, 128), ([5, 0, 0, 7, 1], 264, 272), ([128, 128], 256, 256), ([130, 1, 33, 32, 300], 520, 640),
     ([0] * 63 + [3], 136, 144), ([2] * 300, 72, 128), ([1000, 0, 17], 1032, 528), ([40, 700, 3, 260], 384, 1024),
-    ([1] * 1024, 64, 64),
+    ([1] * 1024, 64, 64), ([513, 255, 256, 1, 0, 700], 264, 272), ([300, 2500], 520, 1296),
 ])
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_grouped(counts, N, K, kind):
