@@ -33,14 +33,11 @@ using namespace ptx;
 
 constexpr int BM = 128;
 constexpr int BK = 128;                      // one scale block of K = one 128-byte swizzle row of e4m3
-constexpr int kSmallRows = 32;               // row box of A for tiles with few rows
-constexpr int kStages = 4;
-constexpr int kStage = 32 * 1024;            // 128 x 128 of A and 128 x 128 of B_T
-constexpr int kRing = kStages * kStage;
+constexpr int kSmallRows = 32;               // row box of A for tiles with few rows, and all of A in the few-rows form
+constexpr int kRingBytes = 200 * 1024;       // operand ring and store boxes
 constexpr int kBoxBytes = 32 * 128;          // a warp's store box: 32 rows of 128 bytes
 constexpr int kBoxes = 2;                    // of them in flight for each epilogue warp
 constexpr int kEpiWarps = 8;
-constexpr int kOutBytes = kEpiWarps * kBoxes * kBoxBytes;
 constexpr int kThreads = 128 + 32 * kEpiWarps;       // 4 warps of control
 constexpr int kAccCols = 128;                // TMEM columns of an accumulator
 constexpr int kAccs = 4;                     // accumulators: all of TMEM
@@ -50,7 +47,7 @@ constexpr int kBarBytes = 1024;
 constexpr int kGroup = 8;                    // scale blocks whose scales are fetched together (one 32-byte sector of a row)
 constexpr int kScaleWords = kGroup * BM + 2 * kGroup;             // of a group: 128 rows', two column blocks'
 constexpr int kScaleBytes = (2 * kScaleWords * 4 + 127) / 128 * 128;
-constexpr int kSmemTotal = 1024 + kRing + kOutBytes + kTableBytes + kScaleBytes + kBarBytes;
+constexpr int kSmemTotal = 1024 + kRingBytes + kTableBytes + kScaleBytes + kBarBytes;
 static_assert(kSmemTotal <= 227 * 1024, "shared memory");
 constexpr int kMaxSplit = 8;
 // Registers of the 256-column form, whose epilogue threads hold 128 sums: the launch has 384 x 168;
@@ -101,8 +98,12 @@ struct TilePos {
     int row0, row_end, col0, expert;
 };
 
-// BN = 256: a pair of CTAs works on 256 x 256 tiles (cta_group::2).  BN = 128: one CTA, 128 x 128 tiles.
-template <int BN, typename OutT>
+// BN = 256: a pair of CTAs works on 256 x 256 tiles (cta_group::2).  BN = 128: one CTA, 128 x 128 tiles, or
+// (ROWS = 32) 32 x 128 ones for products with few rows: A's share of a stage shrinks from 16 to 4 KiB, so that
+// ten stages fit instead of four and the weight streams with 160 KiB of it in flight.  The MMA still takes 128
+// rows; the ones past the 32nd read the bytes behind them in the same stage and land in TMEM lanes that nobody
+// reads.
+template <int BN, int ROWS, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a_small,
                 const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_d, const float* __restrict__ a_scale,
@@ -110,12 +111,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 int* status, int kernel_id) {
     constexpr int CTA_GROUP = BN / 128;
     constexpr int kHalves = BN / kAccCols;                    // accumulators of a block: one for each 128 columns
-    constexpr int kABytes = BM * BK;
+    constexpr int kABytes = ROWS * BK;
+    constexpr bool kFew = ROWS < BM;
     constexpr int kBRows = kAccCols / CTA_GROUP;              // rows of B_T this CTA loads for an accumulator
-    static_assert(kABytes + kHalves * kBRows * BK == kStage, "ring stage");
-    constexpr int kTileRows = BM * CTA_GROUP;
+    constexpr int kStage = kABytes + kHalves * kBRows * BK;
+    constexpr int kOutBytes = kFew ? 0 : kEpiWarps * kBoxes * kBoxBytes;      // few rows are stored directly
+    constexpr int kStages = (kRingBytes - kOutBytes) / kStage;
+    static_assert(kStage >= BM * BK, "the MMA reads 128 rows of A from its stage");
+    constexpr int kTileRows = ROWS * CTA_GROUP;
     constexpr uint32_t kTmemCols = kAccs * kAccCols;
-    constexpr uint32_t kIdesc = make_idesc_e4m3(kTileRows, kAccCols);
+    constexpr uint32_t kIdesc = make_idesc_e4m3(BM * CTA_GROUP, kAccCols);
     constexpr int kCols = BN / 2;                             // columns of an epilogue warp: f32 sums of a thread
     constexpr int kColBlocks = BN / BK;                       // scale blocks of a tile's columns
 
@@ -123,10 +128,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t s_ring = smem_base;
-    const uint32_t s_bar = s_ring + kRing + kOutBytes + kTableBytes + kScaleBytes;
-    int* seg = reinterpret_cast<int*>(smem_gen + kRing + kOutBytes);      // [experts+1] row offsets
+    const uint32_t s_bar = s_ring + kRingBytes + kTableBytes + kScaleBytes;
+    int* seg = reinterpret_cast<int*>(smem_gen + kRingBytes);      // [experts+1] row offsets
     int* seg_tile = seg + kMaxExperts + 1;                    // [experts+1] M-tiles before
-    const uint32_t s_scales = s_ring + kRing + kOutBytes + kTableBytes;      // 2 x ([kGroup][BM] of A, [kColBlocks][kGroup] of B)
+    const uint32_t s_scales = s_ring + kRingBytes + kTableBytes;      // 2 x ([kGroup][BM] of A, [kColBlocks][kGroup] of B)
     const float* scales = reinterpret_cast<const float*>(smem_gen + (s_scales - smem_base));
     const uint32_t bar_full = s_bar, bar_empty = bar_full + 8 * kStages;
     const uint32_t bar_tfull = bar_empty + 8 * kStages, bar_tempty = bar_tfull + 8 * kAccs;
@@ -154,11 +159,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
         for (int b = 0; b < kAccs; ++b) {
             mbar_init(bar_tfull + 8 * b, 1);
-            mbar_init(bar_tempty + 8 * b, kEpiWarps / kHalves * CTA_GROUP);
+            mbar_init(bar_tempty + 8 * b, kFew ? 2 : kEpiWarps / kHalves * CTA_GROUP);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(bar_sfull + 8 * b, 32);
-            mbar_init(bar_sempty + 8 * b, kEpiWarps);
+            mbar_init(bar_sempty + 8 * b, kFew ? 2 : kEpiWarps);
         }
         fence_mbarrier_init();
         fence_proxy_async_smem();
@@ -245,13 +250,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             for (int t = unit; t < n_tiles && ok; t += n_units) {
                 const TilePos p = tile_pos(t);
                 const int row_a = p.row0 + (int)pair_rank * BM;
-                const bool small = p.row_end - row_a <= kSmallRows;
+                const bool small = kFew || p.row_end - row_a <= kSmallRows;
                 const int row_b = p.expert * shape.n + p.col0 + (int)pair_rank * kBRows;      // of the first half
                 // bytes of this CTA's loads, and for the leader of a pair its peer's too
                 uint32_t tx = 0;
 #pragma unroll
                 for (int c = 0; c < CTA_GROUP; ++c)
-                    tx += (uint32_t)((p.row_end - p.row0 - c * BM <= kSmallRows ? kSmallRows * BK : kABytes) + kHalves * kBRows * BK);
+                    tx += (uint32_t)((kFew || p.row_end - p.row0 - c * BM <= kSmallRows ? kSmallRows * BK : kABytes) + kHalves * kBRows * BK);
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1u, ctx, 1))) break;
                     const uint32_t dst = s_ring + stage * kStage, bar = bar_full + 8 * stage;
@@ -327,7 +332,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     if (!ok) break;
                     const uint32_t dst = s_scales + (uint32_t)(buf * kScaleWords + lane) * 4u;
 #pragma unroll 1
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < ROWS / 32; ++j) {
                         const bool there = row0 + 32 * j < p.row_end;
                         const float* sa = a_scale + (there ? (long long)(row0 + 32 * j) * shape.blocks : 0ll);
 #pragma unroll
@@ -344,15 +349,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     } else {
         if (BN == 256) reg_alloc<kEpilogueRegs>();
         const int q = warp & 3, group = (warp - 4) >> 2;
-        const uint32_t box = s_ring + kRing + (uint32_t)(warp - 4) * (kBoxes * kBoxBytes);
+        const bool idle = kFew && q != 0;            // lanes past the 32nd row
+        const uint32_t box = s_ring + kRingBytes - kOutBytes + (uint32_t)(warp - 4) * (kBoxes * kBoxBytes);
         const uint32_t tempty_leader = CTA_GROUP == 2 ? map_to_cta(bar_tempty, 0) : bar_tempty;
         constexpr int kAccStep = kHalves;            // this warp's accumulators: those of its half
         const int acc0 = kHalves == 2 ? group : 0, col_in_acc = kHalves == 2 ? 0 : group * kCols;
         int acc = acc0, sbuf = 0;
         uint32_t acc_phase = 0, sphase = 0;
         bool ok = true;
-        for (int t = unit; t < n_tiles && ok; t += n_units) {
+        for (int t = unit; t < n_tiles && ok && !idle; t += n_units) {
             const TilePos p = tile_pos(t);
+            const int row_limit = kFew ? min(p.row_end, p.row0 + ROWS) : p.row_end;
             const int row = p.row0 + (int)pair_rank * BM + q * 32 + lane;      // this thread's row
             const int col = p.col0 + group * kCols;                   // this warp's first column
             float sum[kCols];
@@ -403,7 +410,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 // One tile a cluster: the ring is drained (every MMA that read it has been waited for
                 // through its accumulator), so the partial tile goes there.
                 float* part = reinterpret_cast<float*>(smem_gen) + (q * 32 + lane) * kPartPitch + group * kCols;
-                if (row < p.row_end) {
+                if (row < row_limit) {
 #pragma unroll
                     for (int i = 0; i < kCols; i += 4)
                         *reinterpret_cast<float4*>(part + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
@@ -413,7 +420,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             constexpr int kBoxCols = 128 / (int)sizeof(OutT);
             const int row_w = p.row0 + (int)pair_rank * BM + q * 32;      // first row of this warp
             // TMA clips a box at the matrix's edges, but not at the end of an expert's rows.
-            const bool whole = shape.experts == 0 || row_w + 32 <= p.row_end;
+            const bool whole = !kFew && (shape.experts == 0 || row_w + 32 <= p.row_end);
 #pragma unroll
             for (int c = 0; c < kCols / kBoxCols; ++c) {
                 uint32_t w[32];
@@ -439,7 +446,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         if (row_w < p.row_end && col + c * kBoxCols < shape.n) tma_store_2d(&tmap_d, buf, col + c * kBoxCols, row_w);
                         tma_store_commit();
                     }
-                } else if (row < p.row_end) {
+                } else if (row < row_limit) {
                     OutT* dst = out + (long long)row * shape.n + col + c * kBoxCols;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -459,7 +466,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         cluster_sync_all();
         if (unit < n_tiles) {
             const TilePos p = tile_pos(unit);
-            const int rows = min(BM, p.row_end - p.row0), vecs = BN / 4;
+            const int rows = min(ROWS, p.row_end - p.row0), vecs = BN / 4;
             uint32_t peer[kMaxSplit];
 #pragma unroll
             for (int s = 0; s < kMaxSplit; ++s) peer[s] = map_to_cta(smem_base, (uint32_t)min(s, split - 1));
@@ -505,17 +512,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 // ---------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Tile shape and split of K.
+//   few rows (32 at most, for each expert on average): 32 x 128 tiles.
+//   dense: 256 x 256 tiles of CTA pairs once they fill the SMs, else 128 x 128 ones.  Where 128-column tiles
+//   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least two blocks
+//   each), which add their partial tiles through distributed shared memory in a fixed order.
+//   grouped: the tiles are known on the device only, so the rows an expert has on average decide.
 struct Plan {
     int64_t experts, m, n, k, tiles;
-    int bn, split;
+    int bn, rows, split;
     int cta_group() const { return bn / 128; }
 };
 
-// Tile width and split of K.
-//   dense: 128 x 256 tiles once they fill the SMs.  With fewer tiles 128-column ones, and where those
-//   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least two
-//   blocks each), which add their partial tiles through distributed shared memory in a fixed order.
-//   grouped: the tiles are known on the device only; 256 columns unless N fits 128.
 Plan make_plan(const Record& r) {
     Plan p{};
     const bool grouped = r.kernel_id == PB200_K_FP8_GROUPED_GEMM;
@@ -523,16 +531,13 @@ Plan make_plan(const Record& r) {
     p.experts = grouped ? r.dims[0] : 0;
     p.m = d[0]; p.n = d[1]; p.k = d[2];
     p.split = 1;
-    const int64_t sms = sm_count(), mt = ceil_div(p.m, BM);
-    if (grouped) {
-        p.bn = p.n > 128 ? 256 : 128;
-        // every expert may end in a partial tile
-        p.tiles = (ceil_div(p.m, BM * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);
-        return p;
-    }
-    p.bn = mt * ceil_div(p.n, 256) >= sms ? 256 : 128;
-    p.tiles = ceil_div(p.m, BM * p.cta_group()) * ceil_div(p.n, p.bn);
-    if (p.bn == 128) {
+    const int64_t sms = sm_count(), mean_rows = grouped ? ceil_div(p.m, p.experts) : p.m;
+    if (mean_rows <= kSmallRows) { p.bn = 128; p.rows = kSmallRows; }
+    else if (grouped ? mean_rows > 128 && p.n > 128 : ceil_div(p.m, BM) * ceil_div(p.n, 256) >= sms) { p.bn = 256; p.rows = BM; }
+    else { p.bn = 128; p.rows = BM; }
+    // every expert may end in a partial tile
+    p.tiles = (ceil_div(p.m, p.rows * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);
+    if (!grouped && p.bn == 128) {
         const int64_t blocks = ceil_div(p.k, BK);
         while (p.split < kMaxSplit && p.tiles * p.split * 2 <= sms && blocks >= 4 * p.split) p.split *= 2;
     }
@@ -545,10 +550,10 @@ int64_t grid_of(const Plan& p) {
     return (p.tiles < most ? p.tiles : most) * cluster;
 }
 
-template <int BN, typename OutT>
+template <int BN, int ROWS, typename OutT>
 int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** ptrs, char* err) {
     constexpr int CTA_GROUP = BN / 128;
-    auto kernel = fp8_gemm_kernel<BN, OutT>;
+    auto kernel = fp8_gemm_kernel<BN, ROWS, OutT>;
     static std::atomic<uint64_t> attr_set{0};   // bit per device
     int dev = 0;
     cudaGetDevice(&dev);
@@ -564,7 +569,7 @@ int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** p
         return make_tensor_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B, err);
     };
     CUtensorMap ta, ta_small, tb;
-    if (int rc = map(&ta, ptrs[0], p.m, BM)) return rc;
+    if (int rc = map(&ta, ptrs[0], p.m, ROWS)) return rc;
     if (int rc = map(&ta_small, ptrs[0], p.m, kSmallRows)) return rc;
     if (int rc = map(&tb, ptrs[2], p.n * (p.experts ? p.experts : 1), kAccCols / CTA_GROUP)) return rc;
     CUtensorMap td;
@@ -579,7 +584,7 @@ int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** p
     s.m = (int)p.m;
     s.n = (int)p.n;
     s.blocks = (int)ceil_div(p.k, BK);
-    s.tiles_m = (int)ceil_div(p.m, BM * CTA_GROUP);
+    s.tiles_m = (int)ceil_div(p.m, ROWS * CTA_GROUP);
     s.tiles_n = (int)ceil_div(p.n, BN);
     s.band = s.tiles_m < 16 ? s.tiles_m : 16;
     s.experts = (int)p.experts;
@@ -631,6 +636,8 @@ int plan_fp8_gemm(Record& r, char* err) {
         return PB200_ERR_BAD_SHAPE;
     }
     pb200_geometry& g = r.geom;
+    g.n_inputs = grouped ? 5 : 4;
+    g.n_outputs = 1;
     g.grid[0] = (uint32_t)grid_of(p);
     g.grid[1] = g.grid[2] = 1;
     g.block[0] = kThreads;
@@ -638,17 +645,22 @@ int plan_fp8_gemm(Record& r, char* err) {
     g.cluster[0] = (uint32_t)(p.split * p.cta_group());
     g.cluster[1] = g.cluster[2] = 1;
     g.smem_bytes = kSmemTotal;
-    g.n_inputs = grouped ? 5 : 4;
-    g.n_outputs = 1;
     return PB200_OK;
 }
 
 int launch_fp8_gemm(const Record& r, cudaStream_t stream, void** ptrs, char* err) {
     const Plan p = make_plan(r);
     const bool b16 = (r.flags & PB200_F_OUT_BF16) != 0;
-    if (p.bn == 256)
-        return b16 ? launch_variant<256, __nv_bfloat16>(r, p, stream, ptrs, err) : launch_variant<256, float>(r, p, stream, ptrs, err);
-    return b16 ? launch_variant<128, __nv_bfloat16>(r, p, stream, ptrs, err) : launch_variant<128, float>(r, p, stream, ptrs, err);
+#define PB200_FP8_CASE(BN_, ROWS_)                                                                  \
+    if (p.bn == BN_ && p.rows == ROWS_)                                                             \
+        return b16 ? launch_variant<BN_, ROWS_, __nv_bfloat16>(r, p, stream, ptrs, err)             \
+                   : launch_variant<BN_, ROWS_, float>(r, p, stream, ptrs, err);
+    PB200_FP8_CASE(256, 128)
+    PB200_FP8_CASE(128, 128)
+    PB200_FP8_CASE(128, 32)
+#undef PB200_FP8_CASE
+    set_err(err, "no fp8 gemm variant for %d x %d tiles", p.rows, p.bn);
+    return PB200_ERR_BAD_SHAPE;
 }
 
 }  // namespace pb200

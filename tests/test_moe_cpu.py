@@ -138,9 +138,10 @@ def test_library_refuses_fp8_gemm(kid, dims, message):
 
 
 def test_fp8_gemm_geometry():
-    """Single tokens split K over a cluster; large products fill the SMs with whole tiles."""
-    one = build_fp8_gemm(1, 4096, 4096)
-    assert one.cluster[0] > 1 and one.grid[0] % one.cluster[0] == 0 and one.scratch_bytes == 0
+    """Products with few tiles split K over a cluster; large ones fill the SMs with whole tiles."""
+    for rows in (1, 64):
+        few = build_fp8_gemm(rows, 4096, 4096)
+        assert few.cluster[0] > 1 and few.grid[0] % few.cluster[0] == 0 and few.scratch_bytes == 0
     big = build_fp8_gemm(8192, 8192, 4096, out_dtype=bf16)
     assert big.cluster == (2, 1, 1) and 100 < big.grid[0] <= 148 and big.smem <= 227 * 1024
     grouped = build_fp8_grouped_gemm_varlen(64, 128, 2048, 2064)
