@@ -37,10 +37,10 @@ constexpr int kSmallRows = 32;               // row box of A for tiles with few 
 constexpr int kRingBytes = 200 * 1024;       // operand ring and store boxes
 constexpr int kBoxBytes = 32 * 128;          // a warp's store box: 32 rows of 128 bytes
 constexpr int kBoxes = 2;                    // of them in flight for each epilogue warp
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 128 + 32 * kEpiWarps;       // 4 warps of control
+constexpr int kLaunchThreads = 384;          // 128-row forms: 4 warps of control, 8 of epilogue
+constexpr int kFewThreads = 256;             // 32-row forms: 3 warps of control, 2 of epilogue (both on lanes 0-31), 3 that only
+                                             // help to add partial tiles (registers are handed out for 8 warps anyway)
 constexpr int kAccCols = 128;                // TMEM columns of an accumulator
-constexpr int kAccs = 4;                     // accumulators: all of TMEM
 constexpr int kMaxExperts = 1024;
 constexpr int kTableBytes = 2 * (kMaxExperts + 1) * 4 + 120;      // sanitised offsets and tile prefix, padded to 128
 constexpr int kBarBytes = 1024;
@@ -48,13 +48,14 @@ constexpr int kGroup = 8;                    // scale blocks whose scales are fe
 constexpr int kScaleWords = kGroup * BM + 2 * kGroup;             // of a group: 128 rows', two column blocks'
 constexpr int kScaleBytes = (2 * kScaleWords * 4 + 127) / 128 * 128;
 constexpr int kSmemTotal = 1024 + kRingBytes + kTableBytes + kScaleBytes + kBarBytes;
+constexpr int kLightRingBytes = 100 * 1024;  // with it two CTAs fit an SM
+constexpr int kPartPitch = 128 + 4;          // f32 row pitch of a split's partial tile: rows on distinct banks
 static_assert(kSmemTotal <= 227 * 1024, "shared memory");
 constexpr int kMaxSplit = 8;
 // Registers of the 256-column form, whose epilogue threads hold 128 sums: the launch has 384 x 168;
 // the control warpgroup gives up 128 x 128 of them and the two epilogue warpgroups take 256 x 64.
 constexpr int kControlRegs = 40, kEpilogueRegs = 232;
-static_assert(128 * kControlRegs + 256 * kEpilogueRegs <= kThreads * 168, "register split");
-constexpr int kPartPitch = 128 + 4;          // f32 row pitch of a split's partial tile: rows on distinct banks
+static_assert(128 * kControlRegs + 256 * kEpilogueRegs <= kLaunchThreads * 168, "register split");
 
 // kind::f8f6f4 with e4m3 operands (format code 0) and f32 accumulation has the same fields as kind::f16.
 constexpr uint32_t make_idesc_e4m3(int m, int n) {
@@ -103,8 +104,10 @@ struct TilePos {
 // ten stages fit instead of four and the weight streams with 160 KiB of it in flight.  The MMA still takes 128
 // rows; the ones past the 32nd read the bytes behind them in the same stage and land in TMEM lanes that nobody
 // reads.
-template <int BN, int ROWS, typename OutT>
-__global__ void __launch_bounds__(kThreads, 1)
+// LIGHT: five stages and half of TMEM, so that the next launch's CTAs set up, and bring their weights into L2,
+// while this launch's finish (dense products of few rows, which a launch's latency would otherwise double).
+template <int BN, int ROWS, bool LIGHT, typename OutT>
+__global__ void __launch_bounds__(ROWS == 32 ? kFewThreads : kLaunchThreads, LIGHT ? 2 : 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a_small,
                 const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_d, const float* __restrict__ a_scale,
                 const float* __restrict__ b_scale, const int* __restrict__ offsets, OutT* __restrict__ out, Shape shape,
@@ -113,10 +116,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     constexpr int kHalves = BN / kAccCols;                    // accumulators of a block: one for each 128 columns
     constexpr int kABytes = ROWS * BK;
     constexpr bool kFew = ROWS < BM;
+    static_assert(!LIGHT || kFew, "the light form has 32 rows");
+    constexpr int kThreads = kFew ? kFewThreads : kLaunchThreads;
+    constexpr int kEpiWarps = kFew ? 2 : 8;
+    constexpr int kAccs = LIGHT ? 2 : 4;                      // accumulators in TMEM
+    constexpr int kRingSpace = LIGHT ? kLightRingBytes : kRingBytes;
+    constexpr int kProducer = kFew ? 2 : 0;                   // warp roles; warp 1 issues MMAs, warp 3 copies scales
     constexpr int kBRows = kAccCols / CTA_GROUP;              // rows of B_T this CTA loads for an accumulator
     constexpr int kStage = kABytes + kHalves * kBRows * BK;
     constexpr int kOutBytes = kFew ? 0 : kEpiWarps * kBoxes * kBoxBytes;      // few rows are stored directly
-    constexpr int kStages = (kRingBytes - kOutBytes) / kStage;
+    static_assert(kRingSpace - kOutBytes >= ROWS * kPartPitch * 4, "partial tile");
+    constexpr int kStages = (kRingSpace - kOutBytes) / kStage;
     static_assert(kStage >= BM * BK, "the MMA reads 128 rows of A from its stage");
     constexpr int kTileRows = ROWS * CTA_GROUP;
     constexpr uint32_t kTmemCols = kAccs * kAccCols;
@@ -128,10 +138,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t s_ring = smem_base;
-    const uint32_t s_bar = s_ring + kRingBytes + kTableBytes + kScaleBytes;
-    int* seg = reinterpret_cast<int*>(smem_gen + kRingBytes);      // [experts+1] row offsets
+    const uint32_t s_bar = s_ring + kRingSpace + (LIGHT ? 0 : kTableBytes) + kScaleBytes;
+    int* seg = reinterpret_cast<int*>(smem_gen + kRingSpace);      // [experts+1] row offsets
     int* seg_tile = seg + kMaxExperts + 1;                    // [experts+1] M-tiles before
-    const uint32_t s_scales = s_ring + kRingBytes + kTableBytes;      // 2 x ([kGroup][BM] of A, [kColBlocks][kGroup] of B)
+    const uint32_t s_scales = s_ring + kRingSpace + (LIGHT ? 0 : kTableBytes);      // 2 x ([kGroup][BM] of A, [kColBlocks][kGroup] of B)
     const float* scales = reinterpret_cast<const float*>(smem_gen + (s_scales - smem_base));
     const uint32_t bar_full = s_bar, bar_empty = bar_full + 8 * kStages;
     const uint32_t bar_tfull = bar_empty + 8 * kStages, bar_tempty = bar_tfull + 8 * kAccs;
@@ -159,11 +169,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
         for (int b = 0; b < kAccs; ++b) {
             mbar_init(bar_tfull + 8 * b, 1);
-            mbar_init(bar_tempty + 8 * b, kFew ? 2 : kEpiWarps / kHalves * CTA_GROUP);
+            mbar_init(bar_tempty + 8 * b, kEpiWarps / kHalves * CTA_GROUP);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(bar_sfull + 8 * b, 32);
-            mbar_init(bar_sempty + 8 * b, kFew ? 2 : kEpiWarps);
+            mbar_init(bar_sempty + 8 * b, kEpiWarps);
         }
         fence_mbarrier_init();
         fence_proxy_async_smem();
@@ -176,8 +186,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         tmem_relinquish<CTA_GROUP>();
     }
     pdl_launch_dependents();
-    pdl_wait();
-    if (shape.experts > 0 && warp == 0) {
+    if (LIGHT && warp == kProducer && lane == 0 && unit < shape.tiles_m * shape.tiles_n) {
+        // The weight does not depend on the previous kernel's results in any way that L2 would not see.
+        const int band_tiles = shape.band * shape.tiles_n, b = unit / band_tiles, r = unit - b * band_tiles;
+        const int row_b = r / min(shape.band, shape.tiles_m - b * shape.band) * BN;
+        for (int kb = kb0; kb < min(kb1, kb0 + 16); ++kb) tma_prefetch_2d(&tmap_b, kb * BK, row_b);
+    }
+    const bool grouped = !LIGHT && shape.experts > 0;
+    if (grouped) pdl_wait();
+    if (grouped && warp == 0) {
         // Row offsets, made non-decreasing and clipped to [0, m] whatever they hold, and the number of
         // M-tiles before each expert; 32 experts at a time.
         int run_max = 0, run_tiles = 0;
@@ -210,12 +227,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     tc_fence_before_sync();
     if (CTA_GROUP == 2) cluster_sync_all(); else __syncthreads();
     tc_fence_after_sync();
+    // Set-up above overlaps the previous kernel's tail; global memory is read and written only below.
+    if (!grouped) pdl_wait();
     const uint32_t tmem_base = *tmem_slot_gen;
-    const int n_tiles = (shape.experts > 0 ? seg_tile[shape.experts] : shape.tiles_m) * shape.tiles_n;
+    const int n_tiles = (grouped ? seg_tile[shape.experts] : shape.tiles_m) * shape.tiles_n;
 
     auto tile_pos = [&](int t) {
         TilePos p;
-        if (shape.experts > 0) {
+        if (grouped) {
             int lo = 0, hi = shape.experts;          // last expert whose first tile is at or before t
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
@@ -240,9 +259,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         return p;
     };
 
-    if (warp < 4) {
+    if (kFew ? warp > 0 && warp < 4 : warp < 4) {
         if (BN == 256) reg_dealloc<kControlRegs>();
-        if (warp == 0 && lane == 0) {
+        if (warp == kProducer && lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
             const uint32_t full_leader = CTA_GROUP == 2 ? map_to_cta(bar_full, 0) : bar_full;
@@ -263,7 +282,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     if (CTA_GROUP == 1) {
                         mbar_arrive_expect_tx(bar, tx);
                         tma_load_2d(dst + kABytes, &tmap_b, bar, kb * BK, row_b);
-                        tma_load_2d(dst, small ? &tmap_a_small : &tmap_a, bar, kb * BK, row_a);
+                        tma_load_2d(dst, !kFew && small ? &tmap_a_small : &tmap_a, bar, kb * BK, row_a);
                     } else {
                         if (pair_rank == 0) mbar_arrive_expect_tx(bar, tx);
 #pragma unroll
@@ -346,18 +365,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             }
             cp_async_wait_all();
         }
-    } else {
+    } else if (!kFew || warp == 0 || warp == 4) {
         if (BN == 256) reg_alloc<kEpilogueRegs>();
-        const int q = warp & 3, group = (warp - 4) >> 2;
-        const bool idle = kFew && q != 0;            // lanes past the 32nd row
-        const uint32_t box = s_ring + kRingBytes - kOutBytes + (uint32_t)(warp - 4) * (kBoxes * kBoxBytes);
+        const int q = warp & 3, group = kFew ? warp >> 2 : (warp - 4) >> 2;      // few rows: warps 0 and 4
+        const uint32_t box = s_ring + kRingSpace - kOutBytes + (kFew ? 0u : (uint32_t)(warp - 4) * (kBoxes * kBoxBytes));
         const uint32_t tempty_leader = CTA_GROUP == 2 ? map_to_cta(bar_tempty, 0) : bar_tempty;
         constexpr int kAccStep = kHalves;            // this warp's accumulators: those of its half
+        static_assert(kAccs % kHalves == 0, "a half's accumulators");
         const int acc0 = kHalves == 2 ? group : 0, col_in_acc = kHalves == 2 ? 0 : group * kCols;
         int acc = acc0, sbuf = 0;
         uint32_t acc_phase = 0, sphase = 0;
         bool ok = true;
-        for (int t = unit; t < n_tiles && ok && !idle; t += n_units) {
+        for (int t = unit; t < n_tiles && ok; t += n_units) {
             const TilePos p = tile_pos(t);
             const int row_limit = kFew ? min(p.row_end, p.row0 + ROWS) : p.row_end;
             const int row = p.row0 + (int)pair_rank * BM + q * 32 + lane;      // this thread's row
@@ -409,11 +428,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             if (split > 1) {
                 // One tile a cluster: the ring is drained (every MMA that read it has been waited for
                 // through its accumulator), so the partial tile goes there.
-                float* part = reinterpret_cast<float*>(smem_gen) + (q * 32 + lane) * kPartPitch + group * kCols;
+                float* mine = reinterpret_cast<float*>(smem_gen) + (q * 32 + lane) * kPartPitch + group * kCols;
                 if (row < row_limit) {
 #pragma unroll
                     for (int i = 0; i < kCols; i += 4)
-                        *reinterpret_cast<float4*>(part + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+                        *reinterpret_cast<float4*>(mine + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
                 }
                 break;
             }
@@ -462,7 +481,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     tc_fence_before_sync();
     if (split > 1) {
         // Sum of the partial tiles, read through distributed shared memory in the order of K: CTA r of the
-        // cluster finishes every split-th vector of the tile.
+        // cluster finishes every split-th vector of the tile.  (Writing the partial sums to the CTA that adds
+        // them needs one barrier less here but one more at the start, and measured 0.6 us slower.)
         cluster_sync_all();
         if (unit < n_tiles) {
             const TilePos p = tile_pos(unit);
@@ -513,14 +533,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tile shape and split of K.
-//   few rows (32 at most, for each expert on average): 32 x 128 tiles.
+//   few rows (32 at most; 16 for each expert on average, since loads are uneven): 32 x 128 tiles.
 //   dense: 256 x 256 tiles of CTA pairs once they fill the SMs, else 128 x 128 ones.  Where 128-column tiles
-//   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least two blocks
-//   each), which add their partial tiles through distributed shared memory in a fixed order.
+//   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least eight blocks
+//   each: the cluster's two barriers take about 1.6 us), which add their partial tiles through distributed shared memory in a fixed order.
 //   grouped: the tiles are known on the device only, so the rows an expert has on average decide.
 struct Plan {
     int64_t experts, m, n, k, tiles;
     int bn, rows, split;
+    bool light;
     int cta_group() const { return bn / 128; }
 };
 
@@ -532,34 +553,39 @@ Plan make_plan(const Record& r) {
     p.m = d[0]; p.n = d[1]; p.k = d[2];
     p.split = 1;
     const int64_t sms = sm_count(), mean_rows = grouped ? ceil_div(p.m, p.experts) : p.m;
-    if (mean_rows <= kSmallRows) { p.bn = 128; p.rows = kSmallRows; }
+    if (mean_rows <= (grouped ? kSmallRows / 2 : kSmallRows)) { p.bn = 128; p.rows = kSmallRows; p.light = !grouped; }
     else if (grouped ? mean_rows > 128 && p.n > 128 : ceil_div(p.m, BM) * ceil_div(p.n, 256) >= sms) { p.bn = 256; p.rows = BM; }
     else { p.bn = 128; p.rows = BM; }
     // every expert may end in a partial tile
     p.tiles = (ceil_div(p.m, p.rows * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);
     if (!grouped && p.bn == 128) {
         const int64_t blocks = ceil_div(p.k, BK);
-        while (p.split < kMaxSplit && p.tiles * p.split * 2 <= sms && blocks >= 4 * p.split) p.split *= 2;
+        const int64_t slots = p.light ? 2 * sms : sms;
+        while (p.split < kMaxSplit && p.tiles * p.split * 2 <= slots && blocks >= 16 * p.split) p.split *= 2;
     }
     return p;
 }
 
 // CTAs of a launch: whole clusters, one for each tile or as many as the SMs hold.
 int64_t grid_of(const Plan& p) {
-    const int64_t cluster = p.split * p.cta_group(), most = p.split > 1 ? p.tiles : sm_count() / p.cta_group();
+    const int64_t cluster = p.split * p.cta_group(), most = p.split > 1 ? p.tiles : sm_count() * (p.light ? 2 : 1) / p.cta_group();
     return (p.tiles < most ? p.tiles : most) * cluster;
 }
 
-template <int BN, int ROWS, typename OutT>
+int smem_of(bool light) { return light ? 1024 + kLightRingBytes + kScaleBytes + kBarBytes : kSmemTotal; }
+int threads_of(int rows) { return rows == kSmallRows ? kFewThreads : kLaunchThreads; }
+
+template <int BN, int ROWS, bool LIGHT, typename OutT>
 int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** ptrs, char* err) {
     constexpr int CTA_GROUP = BN / 128;
-    auto kernel = fp8_gemm_kernel<BN, ROWS, OutT>;
+    auto kernel = fp8_gemm_kernel<BN, ROWS, LIGHT, OutT>;
+    const int smem = smem_of(LIGHT), threads = threads_of(ROWS);
     static std::atomic<uint64_t> attr_set{0};   // bit per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!(attr_set.load(std::memory_order_relaxed) & (1ull << (dev & 63)))) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemTotal);
-        if (e != cudaSuccess) { set_err(err, "cudaFuncSetAttribute(smem=%d): %s", kSmemTotal, cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) { set_err(err, "cudaFuncSetAttribute(smem=%d): %s", smem, cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
         attr_set.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
     }
     auto map = [&](CUtensorMap* m, const void* base, int64_t rows, uint32_t box_rows) {
@@ -592,8 +618,8 @@ int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** p
     s.split = p.split;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid_of(p));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmemTotal;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -640,24 +666,25 @@ int plan_fp8_gemm(Record& r, char* err) {
     g.n_outputs = 1;
     g.grid[0] = (uint32_t)grid_of(p);
     g.grid[1] = g.grid[2] = 1;
-    g.block[0] = kThreads;
+    g.block[0] = (uint32_t)threads_of(p.rows);
     g.block[1] = g.block[2] = 1;
     g.cluster[0] = (uint32_t)(p.split * p.cta_group());
     g.cluster[1] = g.cluster[2] = 1;
-    g.smem_bytes = kSmemTotal;
+    g.smem_bytes = (uint32_t)smem_of(p.light);
     return PB200_OK;
 }
 
 int launch_fp8_gemm(const Record& r, cudaStream_t stream, void** ptrs, char* err) {
     const Plan p = make_plan(r);
     const bool b16 = (r.flags & PB200_F_OUT_BF16) != 0;
-#define PB200_FP8_CASE(BN_, ROWS_)                                                                  \
-    if (p.bn == BN_ && p.rows == ROWS_)                                                             \
-        return b16 ? launch_variant<BN_, ROWS_, __nv_bfloat16>(r, p, stream, ptrs, err)             \
-                   : launch_variant<BN_, ROWS_, float>(r, p, stream, ptrs, err);
-    PB200_FP8_CASE(256, 128)
-    PB200_FP8_CASE(128, 128)
-    PB200_FP8_CASE(128, 32)
+#define PB200_FP8_CASE(BN_, ROWS_, LIGHT_)                                                          \
+    if (p.bn == BN_ && p.rows == ROWS_ && p.light == LIGHT_)                                        \
+        return b16 ? launch_variant<BN_, ROWS_, LIGHT_, __nv_bfloat16>(r, p, stream, ptrs, err)     \
+                   : launch_variant<BN_, ROWS_, LIGHT_, float>(r, p, stream, ptrs, err);
+    PB200_FP8_CASE(256, 128, false)
+    PB200_FP8_CASE(128, 128, false)
+    PB200_FP8_CASE(128, 32, false)
+    PB200_FP8_CASE(128, 32, true)
 #undef PB200_FP8_CASE
     set_err(err, "no fp8 gemm variant for %d x %d tiles", p.rows, p.bn);
     return PB200_ERR_BAD_SHAPE;
