@@ -63,6 +63,10 @@ int launch_moe(const Record& r, cudaStream_t stream, void** ptrs, char* err);
 
 int plan_fp8_gemm(Record& r, char* err);
 int launch_fp8_gemm(const Record& r, cudaStream_t stream, void** ptrs, char* err);
+// The dense product's form for few rows (fp8_gemm_skinny.cu).
+int fp8_skinny_warps(int64_t n, int64_t k);
+int64_t fp8_skinny_grid(int64_t n);
+int launch_fp8_skinny(const Record& r, int64_t m, int64_t n, int64_t k, cudaStream_t stream, void** ptrs, char* err);
 
 // Device-side status word (defined in abi.cu's translation unit of the same
 // library; each .cu that needs it reaches it through report_timeout()).

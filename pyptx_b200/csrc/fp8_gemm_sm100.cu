@@ -48,7 +48,6 @@ constexpr int kGroup = 8;                    // scale blocks whose scales are fe
 constexpr int kScaleWords = kGroup * BM + 2 * kGroup;             // of a group: 128 rows', two column blocks'
 constexpr int kScaleBytes = (2 * kScaleWords * 4 + 127) / 128 * 128;
 constexpr int kSmemTotal = 1024 + kRingBytes + kTableBytes + kScaleBytes + kBarBytes;
-constexpr int kLightRingBytes = 100 * 1024;  // with it two CTAs fit an SM
 constexpr int kPartPitch = 128 + 4;          // f32 row pitch of a split's partial tile: rows on distinct banks
 static_assert(kSmemTotal <= 227 * 1024, "shared memory");
 constexpr int kMaxSplit = 8;
@@ -104,10 +103,8 @@ struct TilePos {
 // ten stages fit instead of four and the weight streams with 160 KiB of it in flight.  The MMA still takes 128
 // rows; the ones past the 32nd read the bytes behind them in the same stage and land in TMEM lanes that nobody
 // reads.
-// LIGHT: five stages and half of TMEM, so that the next launch's CTAs set up, and bring their weights into L2,
-// while this launch's finish (dense products of few rows, which a launch's latency would otherwise double).
-template <int BN, int ROWS, bool LIGHT, typename OutT>
-__global__ void __launch_bounds__(ROWS == 32 ? kFewThreads : kLaunchThreads, LIGHT ? 2 : 1)
+template <int BN, int ROWS, typename OutT>
+__global__ void __launch_bounds__(ROWS == 32 ? kFewThreads : kLaunchThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a_small,
                 const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_d, const float* __restrict__ a_scale,
                 const float* __restrict__ b_scale, const int* __restrict__ offsets, OutT* __restrict__ out, Shape shape,
@@ -116,17 +113,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     constexpr int kHalves = BN / kAccCols;                    // accumulators of a block: one for each 128 columns
     constexpr int kABytes = ROWS * BK;
     constexpr bool kFew = ROWS < BM;
-    static_assert(!LIGHT || kFew, "the light form has 32 rows");
     constexpr int kThreads = kFew ? kFewThreads : kLaunchThreads;
     constexpr int kEpiWarps = kFew ? 2 : 8;
-    constexpr int kAccs = LIGHT ? 2 : 4;                      // accumulators in TMEM
-    constexpr int kRingSpace = LIGHT ? kLightRingBytes : kRingBytes;
+    constexpr int kAccs = 4;                                  // accumulators: all of TMEM
     constexpr int kProducer = kFew ? 2 : 0;                   // warp roles; warp 1 issues MMAs, warp 3 copies scales
     constexpr int kBRows = kAccCols / CTA_GROUP;              // rows of B_T this CTA loads for an accumulator
     constexpr int kStage = kABytes + kHalves * kBRows * BK;
     constexpr int kOutBytes = kFew ? 0 : kEpiWarps * kBoxes * kBoxBytes;      // few rows are stored directly
-    static_assert(kRingSpace - kOutBytes >= ROWS * kPartPitch * 4, "partial tile");
-    constexpr int kStages = (kRingSpace - kOutBytes) / kStage;
+    static_assert(kRingBytes - kOutBytes >= ROWS * kPartPitch * 4, "partial tile");
+    constexpr int kStages = (kRingBytes - kOutBytes) / kStage;
     static_assert(kStage >= BM * BK, "the MMA reads 128 rows of A from its stage");
     constexpr int kTileRows = ROWS * CTA_GROUP;
     constexpr uint32_t kTmemCols = kAccs * kAccCols;
@@ -138,10 +133,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t s_ring = smem_base;
-    const uint32_t s_bar = s_ring + kRingSpace + (LIGHT ? 0 : kTableBytes) + kScaleBytes;
-    int* seg = reinterpret_cast<int*>(smem_gen + kRingSpace);      // [experts+1] row offsets
+    const uint32_t s_bar = s_ring + kRingBytes + kTableBytes + kScaleBytes;
+    int* seg = reinterpret_cast<int*>(smem_gen + kRingBytes);      // [experts+1] row offsets
     int* seg_tile = seg + kMaxExperts + 1;                    // [experts+1] M-tiles before
-    const uint32_t s_scales = s_ring + kRingSpace + (LIGHT ? 0 : kTableBytes);      // 2 x ([kGroup][BM] of A, [kColBlocks][kGroup] of B)
+    const uint32_t s_scales = s_ring + kRingBytes + kTableBytes;      // 2 x ([kGroup][BM] of A, [kColBlocks][kGroup] of B)
     const float* scales = reinterpret_cast<const float*>(smem_gen + (s_scales - smem_base));
     const uint32_t bar_full = s_bar, bar_empty = bar_full + 8 * kStages;
     const uint32_t bar_tfull = bar_empty + 8 * kStages, bar_tempty = bar_tfull + 8 * kAccs;
@@ -186,13 +181,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         tmem_relinquish<CTA_GROUP>();
     }
     pdl_launch_dependents();
-    if (LIGHT && warp == kProducer && lane == 0 && unit < shape.tiles_m * shape.tiles_n) {
-        // The weight does not depend on the previous kernel's results in any way that L2 would not see.
-        const int band_tiles = shape.band * shape.tiles_n, b = unit / band_tiles, r = unit - b * band_tiles;
-        const int row_b = r / min(shape.band, shape.tiles_m - b * shape.band) * BN;
-        for (int kb = kb0; kb < min(kb1, kb0 + 16); ++kb) tma_prefetch_2d(&tmap_b, kb * BK, row_b);
-    }
-    const bool grouped = !LIGHT && shape.experts > 0;
+    const bool grouped = shape.experts > 0;
     if (grouped) pdl_wait();
     if (grouped && warp == 0) {
         // Row offsets, made non-decreasing and clipped to [0, m] whatever they hold, and the number of
@@ -368,7 +357,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     } else if (!kFew || warp == 0 || warp == 4) {
         if (BN == 256) reg_alloc<kEpilogueRegs>();
         const int q = warp & 3, group = kFew ? warp >> 2 : (warp - 4) >> 2;      // few rows: warps 0 and 4
-        const uint32_t box = s_ring + kRingSpace - kOutBytes + (kFew ? 0u : (uint32_t)(warp - 4) * (kBoxes * kBoxBytes));
+        const uint32_t box = s_ring + kRingBytes - kOutBytes + (kFew ? 0u : (uint32_t)(warp - 4) * (kBoxes * kBoxBytes));
         const uint32_t tempty_leader = CTA_GROUP == 2 ? map_to_cta(bar_tempty, 0) : bar_tempty;
         constexpr int kAccStep = kHalves;            // this warp's accumulators: those of its half
         static_assert(kAccs % kHalves == 0, "a half's accumulators");
@@ -533,6 +522,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tile shape and split of K.
+//   8 rows at most, dense: the streaming kernel of fp8_gemm_skinny.cu (1 x 4096 x 4096 from HBM: 5.4 us against
+//   7.4 on 32 x 128 tiles), with 9 to 16 rows up to 16 Mi weights, since its arithmetic doubles (16 x 4096 x 4096:
+//   6.6 against 7.8 us, but 16 x 8192 x 8192: 19.5 against 15).
 //   few rows (32 at most; 16 for each expert on average, since loads are uneven): 32 x 128 tiles.
 //   dense: 256 x 256 tiles of CTA pairs once they fill the SMs, else 128 x 128 ones.  Where 128-column tiles
 //   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least eight blocks
@@ -541,7 +533,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Plan {
     int64_t experts, m, n, k, tiles;
     int bn, rows, split;
-    bool light;
+    bool skinny;
     int cta_group() const { return bn / 128; }
 };
 
@@ -553,39 +545,41 @@ Plan make_plan(const Record& r) {
     p.m = d[0]; p.n = d[1]; p.k = d[2];
     p.split = 1;
     const int64_t sms = sm_count(), mean_rows = grouped ? ceil_div(p.m, p.experts) : p.m;
-    if (mean_rows <= (grouped ? kSmallRows / 2 : kSmallRows)) { p.bn = 128; p.rows = kSmallRows; p.light = !grouped; }
+    if (!grouped && (p.m <= 8 || (p.m <= 16 && p.n * p.k <= (1 << 24)))) {
+        p.skinny = true;
+        p.tiles = fp8_skinny_grid(p.n);
+        return p;
+    }
+    if (mean_rows <= (grouped ? kSmallRows / 2 : kSmallRows)) { p.bn = 128; p.rows = kSmallRows; }
     else if (grouped ? mean_rows > 128 && p.n > 128 : ceil_div(p.m, BM) * ceil_div(p.n, 256) >= sms) { p.bn = 256; p.rows = BM; }
     else { p.bn = 128; p.rows = BM; }
     // every expert may end in a partial tile
     p.tiles = (ceil_div(p.m, p.rows * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);
     if (!grouped && p.bn == 128) {
         const int64_t blocks = ceil_div(p.k, BK);
-        const int64_t slots = p.light ? 2 * sms : sms;
-        while (p.split < kMaxSplit && p.tiles * p.split * 2 <= slots && blocks >= 16 * p.split) p.split *= 2;
+        while (p.split < kMaxSplit && p.tiles * p.split * 2 <= sms && blocks >= 16 * p.split) p.split *= 2;
     }
     return p;
 }
 
 // CTAs of a launch: whole clusters, one for each tile or as many as the SMs hold.
 int64_t grid_of(const Plan& p) {
-    const int64_t cluster = p.split * p.cta_group(), most = p.split > 1 ? p.tiles : sm_count() * (p.light ? 2 : 1) / p.cta_group();
+    const int64_t cluster = p.split * p.cta_group(), most = p.split > 1 ? p.tiles : sm_count() / p.cta_group();
     return (p.tiles < most ? p.tiles : most) * cluster;
 }
 
-int smem_of(bool light) { return light ? 1024 + kLightRingBytes + kScaleBytes + kBarBytes : kSmemTotal; }
 int threads_of(int rows) { return rows == kSmallRows ? kFewThreads : kLaunchThreads; }
 
-template <int BN, int ROWS, bool LIGHT, typename OutT>
+template <int BN, int ROWS, typename OutT>
 int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** ptrs, char* err) {
     constexpr int CTA_GROUP = BN / 128;
-    auto kernel = fp8_gemm_kernel<BN, ROWS, LIGHT, OutT>;
-    const int smem = smem_of(LIGHT), threads = threads_of(ROWS);
+    auto kernel = fp8_gemm_kernel<BN, ROWS, OutT>;
     static std::atomic<uint64_t> attr_set{0};   // bit per device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!(attr_set.load(std::memory_order_relaxed) & (1ull << (dev & 63)))) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) { set_err(err, "cudaFuncSetAttribute(smem=%d): %s", smem, cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemTotal);
+        if (e != cudaSuccess) { set_err(err, "cudaFuncSetAttribute(smem=%d): %s", kSmemTotal, cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
         attr_set.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
     }
     auto map = [&](CUtensorMap* m, const void* base, int64_t rows, uint32_t box_rows) {
@@ -618,8 +612,8 @@ int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** p
     s.split = p.split;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid_of(p));
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(threads_of(ROWS));
+    cfg.dynamicSmemBytes = kSmemTotal;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -664,27 +658,30 @@ int plan_fp8_gemm(Record& r, char* err) {
     pb200_geometry& g = r.geom;
     g.n_inputs = grouped ? 5 : 4;
     g.n_outputs = 1;
+    g.grid[1] = g.grid[2] = g.block[1] = g.block[2] = g.cluster[0] = g.cluster[1] = g.cluster[2] = 1;
+    if (p.skinny) {
+        g.grid[0] = (uint32_t)p.tiles;
+        g.block[0] = (uint32_t)(32 * fp8_skinny_warps(p.n, p.k));
+        return PB200_OK;
+    }
     g.grid[0] = (uint32_t)grid_of(p);
-    g.grid[1] = g.grid[2] = 1;
     g.block[0] = (uint32_t)threads_of(p.rows);
-    g.block[1] = g.block[2] = 1;
     g.cluster[0] = (uint32_t)(p.split * p.cta_group());
-    g.cluster[1] = g.cluster[2] = 1;
-    g.smem_bytes = (uint32_t)smem_of(p.light);
+    g.smem_bytes = kSmemTotal;
     return PB200_OK;
 }
 
 int launch_fp8_gemm(const Record& r, cudaStream_t stream, void** ptrs, char* err) {
     const Plan p = make_plan(r);
+    if (p.skinny) return launch_fp8_skinny(r, p.m, p.n, p.k, stream, ptrs, err);
     const bool b16 = (r.flags & PB200_F_OUT_BF16) != 0;
-#define PB200_FP8_CASE(BN_, ROWS_, LIGHT_)                                                          \
-    if (p.bn == BN_ && p.rows == ROWS_ && p.light == LIGHT_)                                        \
-        return b16 ? launch_variant<BN_, ROWS_, LIGHT_, __nv_bfloat16>(r, p, stream, ptrs, err)     \
-                   : launch_variant<BN_, ROWS_, LIGHT_, float>(r, p, stream, ptrs, err);
-    PB200_FP8_CASE(256, 128, false)
-    PB200_FP8_CASE(128, 128, false)
-    PB200_FP8_CASE(128, 32, false)
-    PB200_FP8_CASE(128, 32, true)
+#define PB200_FP8_CASE(BN_, ROWS_)                                                                  \
+    if (p.bn == BN_ && p.rows == ROWS_)                                                             \
+        return b16 ? launch_variant<BN_, ROWS_, __nv_bfloat16>(r, p, stream, ptrs, err)             \
+                   : launch_variant<BN_, ROWS_, float>(r, p, stream, ptrs, err);
+    PB200_FP8_CASE(256, 128)
+    PB200_FP8_CASE(128, 128)
+    PB200_FP8_CASE(128, 32)
 #undef PB200_FP8_CASE
     set_err(err, "no fp8 gemm variant for %d x %d tiles", p.rows, p.bn);
     return PB200_ERR_BAD_SHAPE;

@@ -220,12 +220,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, 
                  " [%0], [%1, {%3, %4, %5}], [%2];"
                  :: "r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
-// Brings a box into L2.  L2 is where all of the GPU's accesses meet, so this is safe before pdl_wait()
-// too: a line that the previous kernel writes afterwards is updated in place.
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* m, int c0, int c1) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];"
-                 :: "l"(reinterpret_cast<uint64_t>(m)), "r"(c0), "r"(c1) : "memory");
-}
 // 2-CTA pair form: the data lands in this CTA's shared memory, the completion
 // bytes are signalled on `bar_cluster_addr`, which may be the pair leader's barrier.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar_cluster_addr,

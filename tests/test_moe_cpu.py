@@ -138,8 +138,12 @@ def test_library_refuses_fp8_gemm(kid, dims, message):
 
 
 def test_fp8_gemm_geometry():
-    """Products with few tiles split K over a cluster; large ones fill the SMs with whole tiles."""
-    for rows in (1, 64):
+    """Single tokens stream the weight; products with few tiles split K over a cluster; large ones fill the SMs
+    with whole tiles."""
+    one = build_fp8_gemm(1, 4096, 4096)
+    assert one.cluster == (1, 1, 1) and one.grid == (256, 1, 1) and one.block[0] >= 128 and one.scratch_bytes == 0
+    assert build_fp8_gemm(1, 40, 144).block == (64, 1, 1)
+    for rows in (17, 64):
         few = build_fp8_gemm(rows, 4096, 4096)
         assert few.cluster[0] > 1 and few.grid[0] % few.cluster[0] == 0 and few.scratch_bytes == 0
     big = build_fp8_gemm(8192, 8192, 4096, out_dtype=bf16)
