@@ -293,32 +293,41 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const uint64_t da0 = make_desc_kmajor_sw128(s_ring), db0 = make_desc_kmajor_sw128(s_ring + kABytes);
             const uint32_t a_hi = (uint32_t)(da0 >> 32), b_hi = (uint32_t)(db0 >> 32);
             const bool leader = elect_one();
-            bool ok = true;
+            // The tensor pipe holds only a few MMAs, so a look at two barriers between blocks would drain it: the
+            // next barriers are looked at while this half's MMAs execute.
+            bool ok = true, full_seen = false, tempty_seen = false;
             for (int i = 0; i < total && ok; ++i) {
-                ok = mbar_wait(bar_full + 8 * stage, phase, ctx, 3);
+                if (!full_seen) ok = mbar_wait(bar_full + 8 * stage, phase, ctx, 3);
                 const uint32_t a_lo = (uint32_t)da0 + (uint32_t)(stage * (kStage >> 4));
                 const uint32_t b_lo = (uint32_t)db0 + (uint32_t)(stage * (kStage >> 4));
+                const uint32_t empty = bar_empty + 8 * stage;
+                if (++stage == kStages) { stage = 0; phase ^= 1u; }
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h) {
-                    if (ok) ok = mbar_wait(bar_tempty + 8 * acc, acc_phase ^ 1u, ctx, 2);
+                    if (ok && !tempty_seen) ok = mbar_wait(bar_tempty + 8 * acc, acc_phase ^ 1u, ctx, 2);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    const uint32_t d = tmem_base + (uint32_t)(acc * kAccCols);
+                    const uint32_t d = tmem_base + (uint32_t)(acc * kAccCols), tfull = bar_tfull + 8 * acc;
+                    const uint32_t b_half = b_lo + (uint32_t)(h * (kBRows * BK >> 4));
+                    if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
+                    // 32 e4m3 along K = 32 bytes = +2 in the encoded address
                     if (leader) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)      // 32 e4m3 along K = 32 bytes = +2 in the encoded address
-                            umma_f8_ss<CTA_GROUP>(d, a_lo + 2 * j, a_hi, b_lo + (uint32_t)(h * (kBRows * BK >> 4)) + 2 * j, b_hi, kIdesc,
-                                                  j != 0 ? 1u : 0u);
-                        if (CTA_GROUP == 2) umma_commit_pair(bar_tfull + 8 * acc); else umma_commit<1>(bar_tfull + 8 * acc);
+                        umma_f8_ss<CTA_GROUP>(d, a_lo, a_hi, b_half, b_hi, kIdesc, 0u);
+                        umma_f8_ss<CTA_GROUP>(d, a_lo + 2, a_hi, b_half + 2, b_hi, kIdesc, 1u);
+                        umma_f8_ss<CTA_GROUP>(d, a_lo + 4, a_hi, b_half + 4, b_hi, kIdesc, 1u);
+                    }
+                    tempty_seen = mbar_test_wait(bar_tempty + 8 * acc, acc_phase ^ 1u);
+                    if (h == kHalves - 1) full_seen = mbar_test_wait(bar_full + 8 * stage, phase);
+                    if (leader) {
+                        umma_f8_ss<CTA_GROUP>(d, a_lo + 6, a_hi, b_half + 6, b_hi, kIdesc, 1u);
+                        if (CTA_GROUP == 2) umma_commit_pair(tfull); else umma_commit<1>(tfull);
                         if (h == kHalves - 1) {
-                            if (CTA_GROUP == 2) umma_commit_pair(bar_empty + 8 * stage); else umma_commit<1>(bar_empty + 8 * stage);
+                            if (CTA_GROUP == 2) umma_commit_pair(empty); else umma_commit<1>(empty);
                         }
                     }
                     __syncwarp();
-                    if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
                 }
-                if (++stage == kStages) { stage = 0; phase ^= 1u; }
             }
         }
         if (warp == 3) {
