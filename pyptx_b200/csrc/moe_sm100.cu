@@ -91,6 +91,7 @@ template <> struct Vec<__nv_bfloat16> {
 // ---------------------------------------------------------------------------
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteMaxCtas = 8;
 constexpr int kRouteRegRounds = 8;            // rounds whose ids and ranks stay in registers
 
 struct RouteArgs {
@@ -113,8 +114,16 @@ __device__ __forceinline__ int load_id(const void* ids, int i, int n, int expert
 }
 
 // Rank of this lane's entry among the entries of its expert that this warp has seen; advances the counter.
-__device__ __forceinline__ int warp_rank(int* counters, int id, int lane) {
-    const unsigned same = __match_any_sync(0xffffffffu, id);
+// The lanes with the same expert are found with one ballot for each bit of the id (cheaper than
+// match_any, which takes one step for each distinct value).
+__device__ __forceinline__ int warp_rank(int* counters, int id, int lane, int id_bits) {
+    unsigned same = __ballot_sync(0xffffffffu, id >= 0);
+    if (id < 0) same = ~same;
+    for (int b = 0; b < id_bits; ++b) {
+        const bool bit = (id >> b) & 1;
+        const unsigned votes = __ballot_sync(0xffffffffu, bit);
+        same &= bit ? votes : ~votes;
+    }
     const unsigned before = same & ((1u << lane) - 1u);
     int base = 0;
     if (id >= 0) base = counters[id];
@@ -140,6 +149,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n_ctas));
     const int rank = (int)ptx::cluster_ctarank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int id_bits = 32 - __clz(E - 1);          // E = 1: none
     const int first = (rank * kRouteWarps + warp) * a.per_warp;
     const int rounds = first < a.n ? (min(a.per_warp, a.n - first) + 31) / 32 : 0;
 
@@ -153,13 +163,13 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     if (IN_REGS) {
 #pragma unroll
         for (int r = 0; r < kRouteRegRounds; ++r)
-            if (r < rounds) my_rank[r] = warp_rank(counters + warp * E, my_id[r], lane);
+            if (r < rounds) my_rank[r] = warp_rank(counters + warp * E, my_id[r], lane, id_bits);
     } else {
         int next = load_id<IdT>(a.ids, first + lane, rounds > 0 ? a.n : 0, E);
         for (int r = 0; r < rounds; ++r) {
             const int i = first + r * 32 + lane, id = next;
             next = r + 1 < rounds ? load_id<IdT>(a.ids, i + 32, a.n, E) : -1;
-            const int rk = warp_rank(counters + warp * E, id, lane);
+            const int rk = warp_rank(counters + warp * E, id, lane, id_bits);
             if (i < a.n) a.row_of[i] = rk;          // kept for the second pass of this same thread
         }
     }
@@ -180,11 +190,17 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     int total = 0, before = 0;
     if (tid < E) {
         const uint32_t own = ptx::smem_u32(cta_count + tid);
-        for (int c = 0; c < (int)n_ctas; ++c) {
-            int v;
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ptx::map_to_cta(own, (uint32_t)c)) : "memory");
-            if (c < rank) before += v;
-            total += v;
+        int v[kRouteMaxCtas];
+#pragma unroll
+        for (int c = 0; c < kRouteMaxCtas; ++c) {        // all reads in flight at once
+            v[c] = 0;
+            if (c < (int)n_ctas)
+                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[c]) : "r"(ptx::map_to_cta(own, (uint32_t)c)) : "memory");
+        }
+#pragma unroll
+        for (int c = 0; c < kRouteMaxCtas; ++c) {
+            if (c < rank) before += v[c];
+            total += v[c];
         }
     }
     const int padded = (total + a.block - 1) / a.block * a.block;
@@ -588,7 +604,7 @@ int route_ctas(int64_t n) {
     // One CTA ranks 32 entries a warp and round; a second CTA costs a cluster barrier, so the cluster
     // grows only once a CTA would walk more than two rounds.
     int ctas = 1;
-    while (ctas < 8 && n > (int64_t)ctas * 2 * kRouteThreads) ctas *= 2;
+    while (ctas < kRouteMaxCtas && n > (int64_t)ctas * 2 * kRouteThreads) ctas *= 2;
     return ctas;
 }
 size_t route_smem(int64_t experts) { return (size_t)(kRouteWarps + 4) * experts * sizeof(int); }
