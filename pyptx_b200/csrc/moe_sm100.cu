@@ -438,8 +438,10 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(MoveArgs a) {
     }
 }
 
-// 128 x 128 blocks (weights): a CTA of 256 threads holds one block, 8 rows x 8 columns a thread.
-constexpr int kBlockThreads = 256;
+// 128 x 128 blocks (weights): a CTA of 512 threads holds one block, 4 rows x 8 columns a thread.
+constexpr int kBlockThreads = 512;
+constexpr int kBlockSteps = kScaleBlock * kScaleBlock / (8 * kBlockThreads);
+constexpr int kBlockStep = kScaleBlock / kBlockSteps;          // rows between a thread's
 template <typename T>
 __global__ void __launch_bounds__(kBlockThreads) quantize_blocks_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                                         float* __restrict__ scales, int64_t rows, int cols,
@@ -448,12 +450,13 @@ __global__ void __launch_bounds__(kBlockThreads) quantize_blocks_kernel(const T*
     __shared__ float part[kBlockThreads / 32];
     const int64_t row0 = (int64_t)(blockIdx.x / scale_cols) * kScaleBlock + threadIdx.x / 16;
     const int col = (int)(blockIdx.x % scale_cols) * kScaleBlock + (threadIdx.x % 16) * 8;
-    float v[8][8];
+    float v[kBlockSteps][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load8<T>(x + (row0 + 16 * i) * cols + col, row0 + 16 * i < rows && col < cols, v[i]);
+    for (int i = 0; i < kBlockSteps; ++i)
+        load8<T>(x + (row0 + kBlockStep * i) * cols + col, row0 + kBlockStep * i < rows && col < cols, v[i]);
     float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, amax8(v[i]));
+    for (int i = 0; i < kBlockSteps; ++i) m = fmaxf(m, amax8(v[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x / 32] = m;
@@ -463,9 +466,9 @@ __global__ void __launch_bounds__(kBlockThreads) quantize_blocks_kernel(const T*
     for (int i = 1; i < kBlockThreads / 32; ++i) m = fmaxf(m, part[i]);
     const float scale = block_scale(m), inv = __frcp_rn(scale);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (row0 + 16 * i < rows && col < cols)
-            __stcs(reinterpret_cast<uint2*>(q + (row0 + 16 * i) * cols + col), quantize8(v[i], inv));
+    for (int i = 0; i < kBlockSteps; ++i)
+        if (row0 + kBlockStep * i < rows && col < cols)
+            __stcs(reinterpret_cast<uint2*>(q + (row0 + kBlockStep * i) * cols + col), quantize8(v[i], inv));
     if (threadIdx.x == 0) scales[blockIdx.x] = scale;
 }
 
