@@ -158,7 +158,7 @@ def build_torch_ext(force: bool = False) -> str:
         shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))), "include")]      # cuda_runtime_api.h, for the stream type
     libdirs = [d for d in libdirs if os.path.isdir(d) and "cuda" not in d]
     cmd += ["-L" + d for d in libdirs]
-    cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ldl"]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-ldl"]
     cmd += ["-Wl,-rpath," + d for d in libdirs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

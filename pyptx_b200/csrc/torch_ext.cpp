@@ -16,6 +16,7 @@
 // which words the errors.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -90,31 +91,31 @@ public:
         }
     }
 
-    // One tensor, a tuple of tensors, or None when the inputs are not exactly what the specs say.
-    pybind11::object call(const pybind11::tuple& args) const {
+    // A new reference to one tensor, a tuple of tensors, or None when the inputs are not exactly what the specs say.
+    PyObject* call(PyObject* args) const {
         const size_t n_in = in_shapes_.size();
-        if (!g_launch_raw || args.size() != n_in || n_in == 0) return pybind11::none();
+        if (!g_launch_raw || !PyTuple_CheckExact(args) || (size_t)PyTuple_GET_SIZE(args) != n_in || n_in == 0) return decline();
         constexpr size_t kMaxBuffers = 32;
         void* ptrs[kMaxBuffers];
-        if (n_in + out_shapes_.size() > kMaxBuffers) return pybind11::none();
+        if (n_in + out_shapes_.size() > kMaxBuffers) return decline();
         c10::Device device(c10::DeviceType::CPU);
         for (size_t i = 0; i < n_in; ++i) {
-            PyObject* obj = PyTuple_GET_ITEM(args.ptr(), (Py_ssize_t)i);
-            if (!THPVariable_CheckExact(obj)) return pybind11::none();
+            PyObject* obj = PyTuple_GET_ITEM(args, (Py_ssize_t)i);
+            if (!THPVariable_CheckExact(obj)) return decline();
             const at::Tensor& t = THPVariable_Unpack(obj);
             if (!t.is_cuda() || t.layout() != c10::Layout::Strided || t.scalar_type() != in_dtypes_[i] ||
                 t.sizes() != c10::IntArrayRef(in_shapes_[i]) || !t.is_contiguous())
-                return pybind11::none();
+                return decline();
             if (i == 0) device = t.device();
-            else if (t.device() != device) return pybind11::none();
+            else if (t.device() != device) return decline();
             ptrs[i] = t.data_ptr();
         }
-        if (c10::cuda::current_device() != device.index()) return pybind11::none();
+        if (c10::cuda::current_device() != device.index()) return decline();
         const uint64_t stream = (uint64_t)(uintptr_t)c10::cuda::getCurrentCUDAStream(device.index()).stream();
-        std::vector<at::Tensor> outs;
-        outs.reserve(out_shapes_.size());
+        c10::SmallVector<at::Tensor, 4> outs;
         for (size_t i = 0; i < out_shapes_.size(); ++i) {
-            outs.push_back(torch::empty(out_shapes_[i], torch::TensorOptions().dtype(out_dtypes_[i]).device(device)));
+            // torch's caching allocator on the current stream, without the dispatcher
+            outs.push_back(at::Tensor(at::detail::empty_cuda(out_shapes_[i], out_dtypes_[i], device, std::nullopt)));
             ptrs[n_in + i] = outs.back().data_ptr();
         }
         char err[128] = {0};
@@ -125,27 +126,53 @@ public:
         }
         if (rc != 0)
             throw std::runtime_error("pyptx_b200: pb200_launch_raw failed (code " + std::to_string(rc) + "): " + err);
-        if (n_results_ == 1) return pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(outs[0]));
-        pybind11::tuple res(n_results_);
-        for (size_t i = 0; i < n_results_; ++i)
-            PyTuple_SET_ITEM(res.ptr(), (Py_ssize_t)i, THPVariable_Wrap(outs[i]));
+        if (n_results_ == 1) return THPVariable_Wrap(outs[0]);
+        PyObject* res = PyTuple_New((Py_ssize_t)n_results_);
+        if (!res) return nullptr;
+        for (size_t i = 0; i < n_results_; ++i) PyTuple_SET_ITEM(res, (Py_ssize_t)i, THPVariable_Wrap(outs[i]));
         return res;
     }
 
 private:
+    static PyObject* decline() { Py_RETURN_NONE; }
+
     int64_t handle_;
     size_t n_results_ = 0;
     std::vector<std::vector<int64_t>> out_shapes_, in_shapes_;
     std::vector<c10::ScalarType> in_dtypes_, out_dtypes_;
 };
 
+// The launcher as a plain C function of Python (its self is a capsule around the Launcher): no argument
+// conversion on the way in.
+constexpr const char* kCapsule = "pyptx_b200.Launcher";
+
+PyObject* launcher_call(PyObject* self, PyObject* args) {
+    try {
+        return static_cast<const Launcher*>(PyCapsule_GetPointer(self, kCapsule))->call(args);
+    } catch (const c10::Error&) {
+        Py_RETURN_NONE;             // torch refused an input or an allocation, nothing is enqueued: let the checking path say so
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+PyMethodDef launcher_method = {"launch", launcher_call, METH_O,
+                               "check, allocate and launch; None when the inputs need the checking path"};
+
+pybind11::object make_launcher(int64_t handle, std::vector<int64_t> in_dtypes, std::vector<std::vector<int64_t>> in_shapes,
+                               std::vector<int64_t> out_dtypes, std::vector<std::vector<int64_t>> out_shapes, int64_t scratch_bytes) {
+    auto* launcher = new Launcher(handle, std::move(in_dtypes), std::move(in_shapes), std::move(out_dtypes), std::move(out_shapes),
+                                  scratch_bytes);
+    pybind11::object self = pybind11::reinterpret_steal<pybind11::object>(PyCapsule_New(
+        launcher, kCapsule, [](PyObject* c) { delete static_cast<Launcher*>(PyCapsule_GetPointer(c, kCapsule)); }));
+    if (!self) { delete launcher; throw pybind11::error_already_set(); }
+    return pybind11::reinterpret_steal<pybind11::object>(PyCFunction_New(&launcher_method, self.ptr()));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("load_shim", &load_shim, "dlopen the C-ABI library");
     m.def("launch_kernel", &launch_kernel, "allocate outputs and launch a registered kernel");
-    pybind11::class_<Launcher>(m, "Launcher")
-        .def(pybind11::init<int64_t, std::vector<int64_t>, std::vector<std::vector<int64_t>>, std::vector<int64_t>,
-                            std::vector<std::vector<int64_t>>, int64_t>())
-        .def("call", &Launcher::call, "check, allocate and launch; None when the inputs need the checking path");
+    m.def("make_launcher", &make_launcher, "the launch of one kernel object with static shapes, as a function of its inputs' tuple");
 }

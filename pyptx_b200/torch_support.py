@@ -119,9 +119,9 @@ class _Launcher:
         self.fast = None
         if self.ext is not None and self.static_out_shapes is not None and None not in self.in_shapes \
                 and all(d in codes for d in self.in_dtypes):
-            self.fast = self.ext.Launcher(
+            self.fast = self.ext.make_launcher(
                 self.handle_int, [codes[d] for d in self.in_dtypes], [list(s) for s in self.in_shapes],
-                self.out_dtype_codes, [list(s) for s in self.static_out_shapes], self.scratch_bytes).call
+                self.out_dtype_codes, [list(s) for s in self.static_out_shapes], self.scratch_bytes)
 
 
     def call_buffers(self):
