@@ -373,7 +373,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const int acc0 = kHalves == 2 ? group : 0, col_in_acc = kHalves == 2 ? 0 : group * kCols;
         int acc = acc0, sbuf = 0;
         uint32_t acc_phase = 0, sphase = 0;
-        bool ok = true;
+        bool ok = true, seen = false;                // seen: the next accumulator was complete at the last look
         for (int t = unit; t < n_tiles && ok; t += n_units) {
             const TilePos p = tile_pos(t);
             const int row_limit = kFew ? min(p.row_end, p.row0 + ROWS) : p.row_end;
@@ -387,12 +387,19 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 const float* sa = scales + sbuf * kScaleWords + q * 32 + lane;
                 const float* sb = scales + sbuf * kScaleWords + kGroup * BM + group * kCols / BK * kGroup;
                 const int n_blocks = min(kGroup, kb1 - kb);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                float s_next = sa[0] * sb[0];
                 for (int i = 0; i < n_blocks; ++i) {
-                    if (ok) ok = mbar_wait(bar_tfull + 8 * acc, acc_phase, ctx, 4);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
+                    // A block is a chain of latencies for this warp, so whatever can leaves the chain: the scale is
+                    // read a block ahead, and the next accumulator's barrier looked at under the last FMAs.
+                    const float s = s_next;
+                    if (!__all_sync(0xffffffffu, seen)) {
+                        ok = mbar_wait(bar_tfull + 8 * acc, acc_phase, ctx, 4);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                    }
                     tc_fence_after_sync();
-                    const float s = sa[i * BM] * sb[i];
                     const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kAccCols + col_in_acc);
                     constexpr int kChunks = kCols / 32;
                     uint32_t v[2][32];                       // the next 32 columns arrive under the FMAs
@@ -410,13 +417,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                                 if (CTA_GROUP == 2) mbar_arrive_remote(tempty_leader + 8 * acc);
                                 else mbar_arrive(bar_tempty + 8 * acc);
                             }
+                            if ((acc += kAccStep) >= kAccs) { acc = acc0; acc_phase ^= 1u; }
+                            seen = mbar_test_wait(bar_tfull + 8 * acc, acc_phase);
+                            const int next = min(i + 1, n_blocks - 1);
+                            s_next = sa[next * BM] * sb[next];
                         }
 #pragma unroll
                         for (int j = 0; j < 32; j += 2)
                             fma2v(sum[c * 32 + j], sum[c * 32 + j + 1], __uint_as_float(v[c & 1][j]), __uint_as_float(v[c & 1][j + 1]),
                                   s, s, sum[c * 32 + j], sum[c * 32 + j + 1]);
                     }
-                    if ((acc += kAccStep) >= kAccs) { acc = acc0; acc_phase ^= 1u; }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_sempty + 8 * sbuf);
