@@ -142,6 +142,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const uint32_t bar_tfull = bar_empty + 8 * kStages, bar_tempty = bar_tfull + 8 * kAccs;
     const uint32_t bar_sfull = bar_tempty + 8 * kAccs, bar_sempty = bar_sfull + 16;
     const uint32_t s_tmem_slot = bar_sempty + 16, s_abort = s_tmem_slot + 8;
+    int4* tile_at = reinterpret_cast<int4*>(smem_gen + (s_bar - smem_base) + 512);      // [2], beside the scales
     volatile uint32_t* tmem_slot_gen = (volatile uint32_t*)(smem_gen + (s_tmem_slot - smem_base));
     volatile int* abort_gen = (volatile int*)(smem_gen + (s_abort - smem_base));
 
@@ -167,7 +168,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             mbar_init(bar_tempty + 8 * b, kEpiWarps / kHalves * CTA_GROUP);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(bar_sfull + 8 * b, 32);
+            mbar_init(bar_sfull + 8 * b, 33);                // 32 lanes' copies, and the tile's position
             mbar_init(bar_sempty + 8 * b, kEpiWarps);
         }
         fence_mbarrier_init();
@@ -358,6 +359,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     }
                     if (lane < 2 * kGroup) cp_async_4(dst + kGroup * BM * 4u, sb + min(kb + ib, kb1 - 1), b_there);
                     cp_async_arrive(bar_sfull + 8 * buf);
+                    if (lane == 0) {
+                        // the epilogue takes the tile's position from here instead of working it out between tiles
+                        tile_at[buf] = make_int4(p.row0, p.row_end, p.col0, p.expert);
+                        mbar_arrive(bar_sfull + 8 * buf);
+                    }
                     if (++buf == 2) { buf = 0; phase ^= 1u; }
                 }
             }
@@ -375,10 +381,6 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         uint32_t acc_phase = 0, sphase = 0;
         bool ok = true, seen = false;                // seen: the next accumulator was complete at the last look
         for (int t = unit; t < n_tiles && ok; t += n_units) {
-            const TilePos p = tile_pos(t);
-            const int row_limit = kFew ? min(p.row_end, p.row0 + ROWS) : p.row_end;
-            const int row = p.row0 + (int)pair_rank * BM + q * 32 + lane;      // this thread's row
-            const int col = p.col0 + group * kCols;                   // this warp's first column
             float sum[kCols];
 #pragma unroll
             for (int i = 0; i < kCols; ++i) sum[i] = 0.0f;
@@ -428,11 +430,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                                   s, s, sum[c * 32 + j], sum[c * 32 + j + 1]);
                     }
                 }
+                if (kb + kGroup >= kb1) break;               // the tile's last group is handed back below
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_sempty + 8 * sbuf);
                 if (++sbuf == 2) { sbuf = 0; sphase ^= 1u; }
             }
             if (!ok) break;
+            const int4 at = tile_at[sbuf];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_sempty + 8 * sbuf);
+            if (++sbuf == 2) { sbuf = 0; sphase ^= 1u; }
+            const TilePos p{at.x, at.y, at.z, at.w};
+            const int row_limit = kFew ? min(p.row_end, p.row0 + ROWS) : p.row_end;
+            const int row = p.row0 + (int)pair_rank * BM + q * 32 + lane;      // this thread's row
+            const int col = p.col0 + group * kCols;                   // this warp's first column
             if (split > 1) {
                 // One tile a cluster: the ring is drained (every MMA that read it has been waited for
                 // through its accumulator), so the partial tile goes there.
@@ -447,6 +458,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             constexpr int kBoxCols = 128 / (int)sizeof(OutT);
             const int row_w = p.row0 + (int)pair_rank * BM + q * 32;      // first row of this warp
             // TMA clips a box at the matrix's edges, but not at the end of an expert's rows.
+            // A tile's boxes go round the buffers; with fewer boxes than buffers every tile starts at the same one.
+            constexpr int kBoxesBehind = kCols / kBoxCols >= kBoxes ? kBoxes - 1 : 0;
+            static_assert(kBoxesBehind == 0 || kCols / kBoxCols % kBoxes == 0, "a tile ends where it began");
             const bool whole = !kFew && (shape.experts == 0 || row_w + 32 <= p.row_end);
 #pragma unroll
             for (int c = 0; c < kCols / kBoxCols; ++c) {
@@ -462,7 +476,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 }
                 if (whole) {
                     const uint32_t buf = box + (uint32_t)(c % kBoxes) * kBoxBytes;
-                    if (lane == 0) tma_store_wait_read<kBoxes - 1>();      // the store that last read this buffer
+                    if (lane == 0) tma_store_wait_read<kBoxesBehind>();      // the store that last read this buffer
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 8; ++j)

@@ -113,6 +113,20 @@ def test_special_scales_and_values_stay_in_their_rows():
     assert torch.equal(out[keep.cuda()], clean[keep.cuda()])
 
 
+@pytest.mark.parametrize("M,N,K", [(8192, 264, 128), (4096, 520, 64), (16384, 136, 128), (4096, 4096, 128)])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_tiles_in_quick_succession(M, N, K, kind):
+    """One scale block a tile and several tiles a CTA: a tile's results leave through buffers that the next
+    tile fills at once."""
+    a, sa, b, sb = _operands(M, N, K, 11)
+    kernel = build_fp8_gemm(M, N, K, out_dtype=PTX[kind])
+    ins = [t.cuda() for t in (a, sa, b, sb)]
+    first = kernel(*ins)
+    _check(first, a, sa, b, sb, kind)
+    for _ in range(10):
+        assert torch.equal(kernel(*ins), first)
+
+
 def test_repeated_calls_give_the_same_bits():
     for M, N, K in ((1, 1024, 4096), (700, 1024, 512)):
         a, sa, b, sb = (t.cuda() for t in _operands(M, N, K, 1))
