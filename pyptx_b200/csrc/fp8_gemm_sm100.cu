@@ -590,7 +590,10 @@ Plan make_plan(const Record& r) {
     p.tiles = (ceil_div(p.m, p.rows * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);
     if (!grouped && p.bn == 128) {
         const int64_t blocks = ceil_div(p.k, BK);
-        while (p.split < kMaxSplit && p.tiles * p.split * 2 <= sms && blocks >= 16 * p.split) p.split *= 2;
+        // A cluster lives in one GPC, so only so many run at once: 15 of 8 CTAs and 33 of 4 were seen to (a
+        // 16th doubles 32 x 2048 x 8192 from 8.0 to 13.6 us), and GPUs differ in which SMs they have.
+        auto fits = [&](int64_t split) { return p.tiles * split <= (split == 8 ? sms * 3 / 4 : split == 4 ? sms * 7 / 8 : sms); };
+        while (p.split < kMaxSplit && fits(p.split * 2) && blocks >= 16 * p.split) p.split *= 2;
     }
     return p;
 }
