@@ -559,7 +559,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   7.4 on 32 x 128 tiles), with 9 to 16 rows up to 16 Mi weights, since its arithmetic doubles (16 x 4096 x 4096:
 //   6.6 against 7.8 us, but 16 x 8192 x 8192: 19.5 against 15).
 //   few rows (32 at most; 16 for each expert on average, since loads are uneven): 32 x 128 tiles.
-//   dense: 256 x 256 tiles of CTA pairs once they fill the SMs, else 128 x 128 ones.  Where 128-column tiles
+//   dense: 128 x 128 tiles while they fit the SMs at once (512 x 4096 x 4096: 13.4 us, as pairs 16.4), else
+//   256 x 256 tiles of CTA pairs (768 x 4096 x 4096: 17.7 us, in two rounds of 128 x 128 ones 21.6).  Where 128-column tiles
 //   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least eight blocks
 //   each: the cluster's two barriers take about 1.6 us), which add their partial tiles through distributed shared memory in a fixed order.
 //   grouped: the tiles are known on the device only, so the rows an expert has on average decide.
@@ -584,7 +585,7 @@ Plan make_plan(const Record& r) {
         return p;
     }
     if (mean_rows <= (grouped ? kSmallRows / 2 : kSmallRows)) { p.bn = 128; p.rows = kSmallRows; }
-    else if (grouped ? mean_rows > 128 && p.n > 128 : ceil_div(p.m, BM) * ceil_div(p.n, 256) >= sms) { p.bn = 256; p.rows = BM; }
+    else if (grouped ? mean_rows > 128 && p.n > 128 : ceil_div(p.m, BM) * ceil_div(p.n, 128) > sms) { p.bn = 256; p.rows = BM; }
     else { p.bn = 128; p.rows = BM; }
     // every expert may end in a partial tile
     p.tiles = (ceil_div(p.m, p.rows * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);
