@@ -6,18 +6,26 @@
 //
 // The inner sums run on the tensor cores (tcgen05.mma kind::f8f6f4, f32 accumulation in TMEM), one
 // accumulator for each block of K; the scales are f32 and differ from row to row, so the outer sum
-// runs in registers: eight epilogue warps fetch each block's accumulator from TMEM, multiply it by
-// the row's scale times the weight block's and add it to the tile's f32 sums.  128 rows are the 128
-// TMEM lanes, so a thread has one row: one scale for a block of K, and its columns lie in one weight
-// block.
+// runs in registers: the epilogue warps fetch each block's accumulator from TMEM, multiply it by the
+// row's scale times the weight block's and add it to the tile's f32 sums.  128 rows are the 128 TMEM
+// lanes, so a thread has one row: one scale for a block of K, and its columns lie in one weight block.
 //
-// What bounds it: a 128 x 256 x 128 block takes 512 clocks of MMA, and the drain of its accumulator
-// 256 clocks of TMEM reads and 128 of packed FMA issue on each SM sub-partition.  Two accumulators
-// in TMEM let the drain of one block run under the MMAs of the next.
+// What bounds it at large sizes: a CTA's 128 x 256 x 128 block takes 512 clocks of MMA, 512 of operands
+// from L2 (64 bytes a clock), and the drain of its accumulators 286 clocks of each SM sub-partition's
+// TMEM port and FMA pipe.  The three overlap, but the way MMA -> commit -> epilogue -> release -> MMA
+// has 390 clocks of latency besides the work, and TMEM holds two blocks: a block takes 720 clocks, plus
+// 2600 a tile for its store and the restart (8192 x 8192 x 4096: 229 us, 2400 TFLOP/s back to back, tensor
+// pipe 70 % active; 2040 when run for seconds, under the power cap).
+// What brought it there (8192 x 8192 x 4096): pairs of CTAs with four accumulators of 128 columns instead of
+// two of 256, so that a half is released while the other runs; MMAs issued from uniform registers by an
+// elected lane (from a lane's own they issue at 60 clocks each); the next barriers looked at under the
+// current work, in the issuing warp and in the epilogue; scales copied into shared memory a group of
+// blocks ahead (read from global memory by the epilogue they cost 700 clocks a block): 345 -> 229 us.
+// Two issuing warps, and 16 epilogue warps with 64 columns each, measured slower.
 //
-// Structure as the bf16 GEMM's (gemm_sm100.cu): persistent, warp 0 = TMA producer, warp 1 = MMA
-// issuer and TMEM owner, warps 4-11 = epilogue (two for each quarter of the lanes, each with half of
-// the columns).  Bounded waits throughout.
+// Structure as the bf16 GEMM's (gemm_sm100.cu): persistent, one warp = TMA producer, one = MMA issuer and
+// TMEM owner, one copies scales, the epilogue's warps two for each quarter of the lanes, each with half of
+// the columns.  Bounded waits throughout.
 #include "common.cuh"
 #include "ptx.cuh"
 #include "fmha_math.cuh"
@@ -562,8 +570,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   dense: 128 x 128 tiles while they fit the SMs at once (512 x 4096 x 4096: 13.4 us, as pairs 16.4), else
 //   256 x 256 tiles of CTA pairs (768 x 4096 x 4096: 17.7 us, in two rounds of 128 x 128 ones 21.6).  Where 128-column tiles
 //   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least eight blocks
-//   each: the cluster's two barriers take about 1.6 us), which add their partial tiles through distributed shared memory in a fixed order.
-//   grouped: the tiles are known on the device only, so the rows an expert has on average decide.
+//   each: the cluster's two barriers take about 1.6 us), which add their partial tiles through distributed
+//   shared memory in a fixed order.
+//   grouped: the tiles are known on the device only, so the rows an expert has on average decide: pairs above
+//   128 (32 experts, 4096 x 2048: 128 rows 73 us on 128 x 128 tiles, 76 as pairs; 200 rows 96 and 91).
 struct Plan {
     int64_t experts, m, n, k, tiles;
     int bn, rows, split;

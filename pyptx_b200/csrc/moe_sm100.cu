@@ -9,7 +9,10 @@
 // Everything but the sort moves bytes and computes next to nothing, so those kernels are bound by
 // HBM: 16-byte accesses, consecutive lanes on consecutive segments, every independent load issued
 // before the first use, each input read once and each output written once.  No atomics: every sum
-// has a fixed order, so results are the same from run to run.
+// has a fixed order, so results are the same from run to run.  Measured at 8192 tokens x 4 choices over 32
+// experts, 4096 columns, bf16, rows padded to 128 (algorithmic bytes over time, inputs larger than L2):
+// dispatch 6.35 TB/s, dispatch into e4m3 6.25, its gradient 6.6, combine 6.55, its gradient 6.46; a plain
+// copy reaches 6.54.
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -87,7 +90,8 @@ template <> struct Vec<__nv_bfloat16> {
 // over experts; the row of an entry is the sum of the three.  Rows that no entry owns get entry -1
 // in the same launch, so nothing has to be cleared beforehand.
 //
-// Latency-bound: the ids are read once (4 or 8 bytes an entry), the maps written once.
+// Latency-bound: the ids are read once (4 or 8 bytes an entry), the maps written once.  In a chain of
+// graph launches 128 entries take 3.8 us, 32768 (eight CTAs, 32 experts) 7.9 us.
 // ---------------------------------------------------------------------------
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
@@ -336,6 +340,7 @@ __global__ void __launch_bounds__(kThreads) dispatch_kernel(MoveArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// (Quantising 8192 x 8192 bf16 takes 33.2 us = 6.1 TB/s; two steps a warp instead of four 36.9, eight 38.9.)
 // Quantisation of 128-column blocks: s = max(amax / 448, 2^-120), q = e4m3(x * (1 / s)), in f32 with
 // every step rounded to nearest.  2^-120 keeps 1/s finite, so that an all-zero block gives zeros.
 // amax ignores NaN: a NaN stays in its own element; an infinity makes its block's products NaN.

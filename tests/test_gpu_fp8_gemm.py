@@ -98,8 +98,9 @@ def test_dense(M, N, K, kind):
     _check(d, a, sa, b, sb, kind)
 
 
-def test_special_scales_and_values_stay_in_their_rows():
-    M, N, K = 40, 256, 512
+@pytest.mark.parametrize("M", [10, 16, 20, 40])            # streaming, 32-row and 128-row forms
+def test_special_scales_and_values_stay_in_their_rows(M):
+    N, K = 256, 512
     a, sa, b, sb = _operands(M, N, K, 5)
     clean = build_fp8_gemm(M, N, K)(a.cuda(), sa.cuda(), b.cuda(), sb.cuda())
     a2, sa2 = a.float(), sa.clone()
@@ -125,6 +126,31 @@ def test_tiles_in_quick_succession(M, N, K, kind):
     _check(first, a, sa, b, sb, kind)
     for _ in range(10):
         assert torch.equal(kernel(*ins), first)
+
+
+def test_special_weights_stay_in_their_columns():
+    for M in (3, 20, 200):
+        N, K = 384, 256
+        a, sa, b, sb = _operands(M, N, K, 6)
+        clean = build_fp8_gemm(M, N, K)(a.cuda(), sa.cuda(), b.cuda(), sb.cuda())
+        b2, sb2 = b.float(), sb.clone()
+        b2[77, 130] = float("nan")
+        sb2[2, 0] = float("inf")                             # columns 256 .. 383
+        out = build_fp8_gemm(M, N, K)(a.cuda(), sa.cuda(), b2.to(torch.float8_e4m3fn).cuda(), sb2.cuda())
+        assert torch.isnan(out[:, 77]).all() and not torch.isfinite(out[:, 256:]).any()
+        keep = torch.arange(256) != 77
+        assert torch.equal(out[:, :256][:, keep.cuda()], clean[:, :256][:, keep.cuda()])
+
+
+def test_results_beyond_two_to_the_31_elements():
+    M, N, K = 270000, 8192, 128                              # 2.2e9 results
+    g = torch.Generator(device="cuda").manual_seed(3)
+    a = (torch.randn(M, K, generator=g, device="cuda") * 140).clamp(-448, 448).to(torch.float8_e4m3fn)
+    b = (torch.randn(N, K, generator=g, device="cuda") * 140).clamp(-448, 448).to(torch.float8_e4m3fn)
+    sa, sb = torch.rand(M, 1, generator=g, device="cuda"), torch.rand(N // 128, 1, generator=g, device="cuda")
+    d = build_fp8_gemm(M, N, K, out_dtype=bf16)(a, sa, b, sb)
+    for rows in (slice(0, 64), slice(262100, 262200), slice(M - 70, M)):
+        _check(d[rows], a[rows].cpu(), sa[rows].cpu(), b.cpu(), sb.cpu(), "bf16")
 
 
 def test_repeated_calls_give_the_same_bits():
@@ -160,6 +186,14 @@ def _grouped(counts, N, K, kind, capacity=None, first=0):
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_grouped(counts, N, K, kind):
     _grouped(counts, N, K, kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("counts,N,K", [([128] * 40, 1024, 128), ([96, 32, 128] * 20, 640, 64), ([700, 300] * 4, 2048, 128)])
+def test_grouped_tiles_in_quick_succession(counts, N, K, kind):
+    """As above for the grouped forms: 128-column tiles (128 rows an expert and fewer) and CTA pairs."""
+    for _ in range(3):
+        _grouped(counts, N, K, kind)
 
 
 def test_grouped_leaves_rows_outside_the_offsets_alone():

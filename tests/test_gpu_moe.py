@@ -174,6 +174,34 @@ def test_maps_that_point_outside_are_ignored():
     assert ((d_w.cpu().double() - want_w).abs() <= H * U32 * mag_w).all()
 
 
+def test_rows_beyond_two_to_the_31_elements():
+    """2.2e9 elements of sorted rows: the last ones are addressed with 64-bit offsets in every direction."""
+    T, k, R, H = 6, 2, 540000, 4096
+    row_of = torch.tensor([[0, 539999], [524287, 524288], [3, 4], [539998, 1], [300000, 2], [-1, 400000]], dtype=torch.int32)
+    entry_of = torch.full((R,), -1, dtype=torch.int32)
+    for i, r in enumerate(row_of.reshape(-1).tolist()):
+        if r >= 0:
+            entry_of[r] = i
+    row_of, entry_of = row_of.cuda(), entry_of.cuda()
+    x, w = torch.randn(T, H).to(torch.bfloat16).cuda(), torch.rand(T, k).cuda()
+    rows = moe.build_moe_dispatch(T, k, R, H)(x, row_of, entry_of)
+    for t in range(T):
+        for j in range(k):
+            if row_of[t, j] >= 0:
+                assert torch.equal(rows[int(row_of[t, j])], x[t])
+    assert (rows[539990:539998] == 0).all() and (rows[524289:524400] == 0).all()
+    dx = moe.build_moe_dispatch_bwd(T, k, R, H)(row_of, rows)
+    kept = (row_of >= 0).sum(dim=1, keepdim=True)
+    assert torch.equal(dx, (x.float() * kept).to(torch.bfloat16))
+    d_rows, d_w = moe.build_moe_combine_bwd(T, k, R, H)(rows, w, row_of, entry_of, x)
+    assert torch.equal(d_rows[539999].float(), (w[0, 1] * x[0].float()).to(torch.bfloat16).float())
+    assert (d_w[5, 0] == 0) and (d_w[5, 1] - x[5].double().square().sum()).abs() <= H * U32 * x[5].double().square().sum()
+    q, scale = moe.build_moe_dispatch_fp8(T, k, R, H)(x, row_of, entry_of)
+    wq, ws = formulas.fp8_quantize_ref(x.cpu(), 1)
+    assert torch.equal(q[539999].cpu().double(), wq[0]) and torch.equal(scale[539998].cpu().double(), ws[3])
+    assert (q[524289:524400].float() == 0).all() and (scale[524289:524400] == 0).all()
+
+
 # ---- quantisation ----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("M,K", [(1, 16), (1, 4096), (3, 144), (127, 272), (129, 2064), (1000, 1040), (5000, 256)])
