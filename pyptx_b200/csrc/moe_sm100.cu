@@ -82,7 +82,7 @@ template <> struct Vec<__nv_bfloat16> {
 // Route: a stable counting sort in one launch of one cluster.
 //
 // Entry i = t*k + j asks for expert ids[i].  CTA c of the cluster owns a contiguous range of
-// entries and each of its warps a contiguous part of that, so "earlier entry" is "earlier round of
+// entries and each of its warps a contiguous part of that, so "earlier entry" is "earlier step of
 // the same warp, or an earlier warp, or an earlier CTA".  A warp walks its part 32 entries at a
 // time; match_any gives each lane its rank among the lanes with the same expert, and the warp's
 // running counters in shared memory the rest.  Counters are then prefix-summed over warps (each
@@ -96,7 +96,7 @@ template <> struct Vec<__nv_bfloat16> {
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteMaxCtas = 8;
-constexpr int kRouteRegRounds = 8;            // rounds whose ids and ranks stay in registers
+constexpr int kRouteRegSteps = 8;            // steps whose ids and ranks stay in registers
 
 struct RouteArgs {
     const void* ids;
@@ -155,24 +155,24 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int id_bits = 32 - __clz(E - 1);          // E = 1: none
     const int first = (rank * kRouteWarps + warp) * a.per_warp;
-    const int rounds = first < a.n ? (min(a.per_warp, a.n - first) + 31) / 32 : 0;
+    const int steps = first < a.n ? (min(a.per_warp, a.n - first) + 31) / 32 : 0;
 
-    int my_id[kRouteRegRounds], my_rank[kRouteRegRounds];
+    int my_id[kRouteRegSteps], my_rank[kRouteRegSteps];
     if (IN_REGS) {
 #pragma unroll
-        for (int r = 0; r < kRouteRegRounds; ++r) my_id[r] = r < rounds ? load_id<IdT>(a.ids, first + r * 32 + lane, a.n, E) : -1;
+        for (int r = 0; r < kRouteRegSteps; ++r) my_id[r] = r < steps ? load_id<IdT>(a.ids, first + r * 32 + lane, a.n, E) : -1;
     }
     for (int i = tid; i < kRouteWarps * E; i += kRouteThreads) counters[i] = 0;
     __syncthreads();
     if (IN_REGS) {
 #pragma unroll
-        for (int r = 0; r < kRouteRegRounds; ++r)
-            if (r < rounds) my_rank[r] = warp_rank(counters + warp * E, my_id[r], lane, id_bits);
+        for (int r = 0; r < kRouteRegSteps; ++r)
+            if (r < steps) my_rank[r] = warp_rank(counters + warp * E, my_id[r], lane, id_bits);
     } else {
-        int next = load_id<IdT>(a.ids, first + lane, rounds > 0 ? a.n : 0, E);
-        for (int r = 0; r < rounds; ++r) {
+        int next = load_id<IdT>(a.ids, first + lane, steps > 0 ? a.n : 0, E);
+        for (int r = 0; r < steps; ++r) {
             const int i = first + r * 32 + lane, id = next;
-            next = r + 1 < rounds ? load_id<IdT>(a.ids, i + 32, a.n, E) : -1;
+            next = r + 1 < steps ? load_id<IdT>(a.ids, i + 32, a.n, E) : -1;
             const int rk = warp_rank(counters + warp * E, id, lane, id_bits);
             if (i < a.n) a.row_of[i] = rk;          // kept for the second pass of this same thread
         }
@@ -249,13 +249,13 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     };
     if (IN_REGS) {
 #pragma unroll
-        for (int r = 0; r < kRouteRegRounds; ++r) {
+        for (int r = 0; r < kRouteRegSteps; ++r) {
             const int i = first + r * 32 + lane;
-            if (r < rounds && i < a.n) place(i, my_id[r], my_rank[r]);
+            if (r < steps && i < a.n) place(i, my_id[r], my_rank[r]);
         }
     } else {
 #pragma unroll 4
-        for (int r = 0; r < rounds; ++r) {
+        for (int r = 0; r < steps; ++r) {
             const int i = first + r * 32 + lane;
             if (i < a.n) place(i, load_id<IdT>(a.ids, i, a.n, E), a.row_of[i]);
         }
@@ -615,8 +615,8 @@ __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(MoveArgs a) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int route_ctas(int64_t n) {
-    // One CTA ranks 32 entries a warp and round; a second CTA costs a cluster barrier, so the cluster
-    // grows only once a CTA would walk more than two rounds.
+    // One CTA ranks 32 entries a warp and step; a second CTA costs a cluster barrier, so the cluster
+    // grows only once a CTA would walk more than two steps.
     int ctas = 1;
     while (ctas < kRouteMaxCtas && n > (int64_t)ctas * 2 * kRouteThreads) ctas *= 2;
     return ctas;
@@ -655,7 +655,7 @@ int launch_route(const Record& r, cudaStream_t stream, void** p, char* err) {
     a.rows = (int)r.dims[4];
     const int ctas = (int)r.geom.cluster[0];
     a.per_warp = (int)(ceil_div(ceil_div(n, ctas * kRouteWarps), 32) * 32);
-    auto kernel = a.per_warp <= 32 * kRouteRegRounds ? route_kernel<IdT, true> : route_kernel<IdT, false>;
+    auto kernel = a.per_warp <= 32 * kRouteRegSteps ? route_kernel<IdT, true> : route_kernel<IdT, false>;
     const size_t smem = route_smem(a.experts);
     cudaError_t e = cudaSuccess;
     if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
