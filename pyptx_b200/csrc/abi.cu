@@ -141,9 +141,17 @@ int make_tensor_map(CUtensorMap* out, CUtensorMapDataType dt, int rank, const vo
     cuuint64_t gdim[5]; cuuint64_t gstr[4]; cuuint32_t bx[5]; cuuint32_t es[5];
     for (int i = 0; i < rank; ++i) { gdim[i] = dims[i]; bx[i] = box[i]; es[i] = 1; }
     for (int i = 0; i + 1 < rank; ++i) gstr[i] = strides_bytes[i];
-    CUresult rc = fn(out, dt, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstr, bx, es,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return fn(out, dt, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult rc = encode();
+    if (rc == CUDA_ERROR_INVALID_CONTEXT) {
+        // A host thread whose first CUDA call this is has no context yet (the runtime binds one on the first call
+        // that needs it, the driver does not): bind the current device's.
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) rc = encode(); else cudaGetLastError();
+    }
     if (rc != CUDA_SUCCESS) {
         set_err(err, "cuTensorMapEncodeTiled failed (CUresult %d) rank=%d dim0=%llu box0=%u", (int)rc, rank,
                 (unsigned long long)dims[0], box[0]);

@@ -84,7 +84,7 @@ template <> struct Vec<__nv_bfloat16> {
 // Entry i = t*k + j asks for expert ids[i].  CTA c of the cluster owns a contiguous range of
 // entries and each of its warps a contiguous part of that, so "earlier entry" is "earlier step of
 // the same warp, or an earlier warp, or an earlier CTA".  A warp walks its part 32 entries at a
-// time; match_any gives each lane its rank among the lanes with the same expert, and the warp's
+// time; ballots give each lane its rank among the lanes with the same expert, and the warp's
 // running counters in shared memory the rest.  Counters are then prefix-summed over warps (each
 // thread one expert), over CTAs (through distributed shared memory) and, padded to `block` rows,
 // over experts; the row of an entry is the sum of the three.  Rows that no entry owns get entry -1

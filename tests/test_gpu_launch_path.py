@@ -100,3 +100,39 @@ def test_side_stream_and_threads():
         assert len(outs) == 50
         for out in outs:
             assert all(torch.equal(a, b) for a, b in zip(out, want[n]))
+
+
+@pytest.mark.parametrize("kind", ["gemm", "fp8_gemm", "rms_norm"])
+def test_a_thread_whose_first_cuda_call_is_a_launch(kind):
+    """The raw entry from a host thread that has made no CUDA call (and so has no context bound)."""
+    import threading
+
+    from pyptx_b200.examples.blackwell.fp8_gemm import build_fp8_gemm
+    from pyptx_b200.examples.blackwell.gemm_highperf_blackwell import build_gemm
+
+    if kind == "gemm":
+        k, ins = build_gemm(128, 256, 64), [torch.ones(128, 64, device="cuda").bfloat16(), torch.ones(256, 64, device="cuda").bfloat16()]
+    elif kind == "fp8_gemm":
+        one = torch.ones(64, 128, device="cuda")
+        k, ins = build_fp8_gemm(64, 64, 128), [one.to(torch.float8_e4m3fn), one[:, :1].contiguous(), one.to(torch.float8_e4m3fn),
+                                              torch.ones(1, 1, device="cuda")]
+    else:
+        k, ins = build_rms_norm(16, 512), [torch.ones(16, 512, device="cuda"), torch.ones(512, device="cuda")]
+    want = k(*ins)
+    out = torch.zeros_like(want)
+    ptrs = [t.data_ptr() for t in ins] + [out.data_ptr()]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work():
+        try:
+            _native.launch_raw(k.handle, 0, ptrs)
+        except Exception as exc:  # noqa: BLE001
+            errors.append(exc)
+
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert torch.equal(out, want)
