@@ -96,6 +96,8 @@ template <> struct Vec<__nv_bfloat16> {
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteMaxCtas = 8;
+constexpr int kMaxIdBits = 10;                // ids below kMaxExperts
+static_assert(1 << kMaxIdBits >= kMaxExperts, "id bits");
 constexpr int kRouteRegSteps = 8;            // steps whose ids and ranks stay in registers
 
 struct RouteArgs {
@@ -123,7 +125,9 @@ __device__ __forceinline__ int load_id(const void* ids, int i, int n, int expert
 __device__ __forceinline__ int warp_rank(int* counters, int id, int lane, int id_bits) {
     unsigned same = __ballot_sync(0xffffffffu, id >= 0);
     if (id < 0) same = ~same;
-    for (int b = 0; b < id_bits; ++b) {
+#pragma unroll
+    for (int b = 0; b < kMaxIdBits; ++b) {
+        if (b >= id_bits) break;
         const bool bit = (id >> b) & 1;
         const unsigned votes = __ballot_sync(0xffffffffu, bit);
         same &= bit ? votes : ~votes;
@@ -147,7 +151,9 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     int* base = cta_count + E;                      // [E] first row of this CTA's entries of an expert
     int* filled = base + E;                         // [E] end of the expert's entries (row)
     int* ends = filled + E;                         // [E] end of the expert's rows
-    __shared__ int warp_total[kRouteWarps];
+    int* local = ends + E;                          // [E] first place of an expert among this CTA's sorted entries
+    int2* sorted = reinterpret_cast<int2*>(local + E + (E & 1));      // IN_REGS: (row, entry) of this CTA's entries, by expert
+    __shared__ int warp_total[kRouteWarps], warp_own[kRouteWarps];
 
     uint32_t n_ctas;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n_ctas));
@@ -191,8 +197,9 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     }
     if (n_ctas > 1) ptx::cluster_sync_all(); else __syncthreads();
     // totals over CTAs, then a block-wide exclusive prefix of the padded totals (E <= 1024 threads)
-    int total = 0, before = 0;
+    int total = 0, before = 0, own_count = 0;
     if (tid < E) {
+        own_count = cta_count[tid];
         const uint32_t own = ptx::smem_u32(cta_count + tid);
         int v[kRouteMaxCtas];
 #pragma unroll
@@ -208,26 +215,28 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
         }
     }
     const int padded = (total + a.block - 1) / a.block * a.block;
-    int incl = padded;
+    int incl = padded, own = own_count;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
+        const int v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, own, o);
+        if (lane >= o) { incl += v; own += u; }
     }
-    if (lane == 31) warp_total[warp] = incl;
+    if (lane == 31) { warp_total[warp] = incl; warp_own[warp] = own; }
     __syncthreads();
-    if (warp == 0) {
-        int v = warp_total[lane];
+    if (warp < 2) {
+        int* totals = warp == 0 ? warp_total : warp_own;
+        int v = totals[lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
-        warp_total[lane] = v;
+        totals[lane] = v;
     }
     __syncthreads();
     const int end = incl + (warp > 0 ? warp_total[warp - 1] : 0);
     if (tid < E) {
+        local[tid] = own - own_count + (warp > 0 ? warp_own[warp - 1] : 0);
         const int start = end - padded;
         base[tid] = start + before;
         filled[tid] = start + total;
@@ -238,26 +247,40 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
         }
     }
     __syncthreads();
-    // entries
-    auto place = [&](int i, int id, int rk) {
-        int row = -1;
-        if (id >= 0) {
-            row = base[id] + counters[warp * E + id] + rk;
-            if (row < a.rows) a.entry_of[row] = i; else row = -1;      // no room: dropped
-        }
-        a.row_of[i] = row;
-    };
     if (IN_REGS) {
+        // Entries go to entry_of by way of shared memory, sorted, so that neighbouring lanes store neighbouring
+        // rows (stored straight from the lanes they cost a sector each, and eight SMs store one a clock).
 #pragma unroll
         for (int r = 0; r < kRouteRegSteps; ++r) {
-            const int i = first + r * 32 + lane;
-            if (r < steps && i < a.n) place(i, my_id[r], my_rank[r]);
+            const int i = first + r * 32 + lane, id = my_id[r];
+            if (r < steps && i < a.n) {
+                int row = -1;
+                if (id >= 0) {
+                    const int k = counters[warp * E + id] + my_rank[r];
+                    row = base[id] + k;
+                    if (row >= a.rows) row = -1;                        // no room: dropped
+                    sorted[local[id] + k] = make_int2(row, i);
+                }
+                a.row_of[i] = row;
+            }
+        }
+        __syncthreads();
+        for (int k = tid; k < warp_own[kRouteWarps - 1]; k += kRouteThreads) {
+            const int2 at = sorted[k];
+            if (at.x >= 0) a.entry_of[at.x] = at.y;
         }
     } else {
 #pragma unroll 4
         for (int r = 0; r < steps; ++r) {
             const int i = first + r * 32 + lane;
-            if (i < a.n) place(i, load_id<IdT>(a.ids, i, a.n, E), a.row_of[i]);
+            if (i >= a.n) continue;
+            const int id = load_id<IdT>(a.ids, i, a.n, E);
+            int row = -1;
+            if (id >= 0) {
+                row = base[id] + counters[warp * E + id] + a.row_of[i];
+                if (row < a.rows) a.entry_of[row] = i; else row = -1;
+            }
+            a.row_of[i] = row;
         }
     }
     // rows without an entry: each expert's padding, then everything behind the last expert
@@ -621,7 +644,12 @@ int route_ctas(int64_t n) {
     while (ctas < kRouteMaxCtas && n > (int64_t)ctas * 2 * kRouteThreads) ctas *= 2;
     return ctas;
 }
-size_t route_smem(int64_t experts) { return (size_t)(kRouteWarps + 4) * experts * sizeof(int); }
+int64_t route_per_warp(int64_t n, int ctas) { return ceil_div(ceil_div(n, ctas * kRouteWarps), 32) * 32; }
+bool route_in_regs(int64_t n, int ctas) { return route_per_warp(n, ctas) <= 32 * kRouteRegSteps; }
+size_t route_smem(int64_t n, int64_t experts, int ctas) {
+    const size_t tables = ((size_t)(kRouteWarps + 5) * experts + (experts & 1)) * sizeof(int);
+    return tables + (route_in_regs(n, ctas) ? (size_t)route_per_warp(n, ctas) * kRouteWarps * sizeof(int2) : 0);
+}
 
 bool is_bf16(const Record& r) { return (r.flags & PB200_F_OUT_BF16) != 0; }
 
@@ -654,9 +682,9 @@ int launch_route(const Record& r, cudaStream_t stream, void** p, char* err) {
     a.block = (int)r.dims[3];
     a.rows = (int)r.dims[4];
     const int ctas = (int)r.geom.cluster[0];
-    a.per_warp = (int)(ceil_div(ceil_div(n, ctas * kRouteWarps), 32) * 32);
-    auto kernel = a.per_warp <= 32 * kRouteRegSteps ? route_kernel<IdT, true> : route_kernel<IdT, false>;
-    const size_t smem = route_smem(a.experts);
+    a.per_warp = (int)route_per_warp(n, ctas);
+    auto kernel = route_in_regs(n, ctas) ? route_kernel<IdT, true> : route_kernel<IdT, false>;
+    const size_t smem = route_smem(n, a.experts, ctas);
     cudaError_t e = cudaSuccess;
     if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) {
@@ -743,7 +771,7 @@ int plan_moe(Record& r, char* err) {
         if (rows % block != 0) { set_err(err, "rows=%lld must be divisible by block=%lld", (long long)rows, (long long)block); return PB200_ERR_BAD_SHAPE; }
         g.cluster[0] = g.grid[0] = (uint32_t)route_ctas(T * k);
         g.block[0] = kRouteThreads;
-        g.smem_bytes = (uint32_t)route_smem(E);
+        g.smem_bytes = (uint32_t)route_smem(T * k, E, route_ctas(T * k));
         g.n_inputs = 1;
         g.n_outputs = 3;
         return PB200_OK;
