@@ -62,7 +62,7 @@ constexpr int kMaxSplit = 8;
 // Registers of the 256-column form, whose epilogue threads hold 128 sums: the launch has 384 x 168;
 // the control warpgroup gives up 128 x 128 of them and the two epilogue warpgroups take 256 x 64.
 constexpr int kControlRegs = 40, kEpilogueRegs = 232;
-static_assert(128 * kControlRegs + 256 * kEpilogueRegs <= kLaunchThreads * 168, "register split");
+static_assert(128 * kControlRegs + 256 * kEpilogueRegs <= kLaunchThreads * 168, "register split");     // checked at the first launch too
 
 // kind::f8f6f4 with e4m3 operands (format code 0) and f32 accumulation has the same fields as kind::f16.
 constexpr uint32_t make_idesc_e4m3(int m, int n) {
@@ -568,10 +568,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   6.6 against 7.8 us, but 16 x 8192 x 8192: 19.5 against 15).
 //   few rows (32 at most; 16 for each expert on average, since loads are uneven): 32 x 128 tiles.
 //   dense: 128 x 128 tiles while they fit the SMs at once (512 x 4096 x 4096: 13.4 us, as pairs 16.4), else
-//   256 x 256 tiles of CTA pairs (768 x 4096 x 4096: 17.7 us, in two rounds of 128 x 128 ones 21.6).  Where 128-column tiles
-//   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least eight blocks
-//   each: the cluster's two barriers take about 1.6 us), which add their partial tiles through distributed
-//   shared memory in a fixed order.
+//   256 x 256 tiles of CTA pairs (768 x 4096 x 4096: 17.7 us, as 128 x 128 ones one after the other 21.6),
+//   unless a pair's tile would be half empty (N <= 128).  Where 128-column tiles leave SMs idle the K blocks of
+//   a tile are shared by a cluster of up to 8 CTAs (at least eight blocks each: the cluster's two barriers
+//   take about 1.6 us), which add their partial tiles through distributed shared memory in a fixed order.
 //   grouped: the tiles are known on the device only, so the rows an expert has on average decide: pairs above
 //   128 (32 experts, 4096 x 2048: 128 rows 73 us on 128 x 128 tiles, 76 as pairs; 200 rows 96 and 91).
 struct Plan {
@@ -595,7 +595,7 @@ Plan make_plan(const Record& r) {
         return p;
     }
     if (mean_rows <= (grouped ? kSmallRows / 2 : kSmallRows)) { p.bn = 128; p.rows = kSmallRows; }
-    else if (grouped ? mean_rows > 128 && p.n > 128 : ceil_div(p.m, BM) * ceil_div(p.n, 128) > sms) { p.bn = 256; p.rows = BM; }
+    else if (p.n > 128 && (grouped ? mean_rows > 128 : ceil_div(p.m, BM) * ceil_div(p.n, 128) > sms)) { p.bn = 256; p.rows = BM; }
     else { p.bn = 128; p.rows = BM; }
     // every expert may end in a partial tile
     p.tiles = (ceil_div(p.m, p.rows * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);
@@ -627,6 +627,13 @@ int launch_variant(const Record& r, const Plan& p, cudaStream_t stream, void** p
     if (!(attr_set.load(std::memory_order_relaxed) & (1ull << (dev & 63)))) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemTotal);
         if (e != cudaSuccess) { set_err(err, "cudaFuncSetAttribute(smem=%d): %s", kSmemTotal, cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
+        // The register split of the 256-column form draws on what the launch gets; with fewer it would wait for ever.
+        cudaFuncAttributes fa{};
+        e = cudaFuncGetAttributes(&fa, kernel);
+        if (e != cudaSuccess || (BN == 256 && fa.numRegs * kLaunchThreads < 128 * kControlRegs + 256 * kEpilogueRegs)) {
+            set_err(err, "fp8 gemm: %d registers a thread are too few for its register split", fa.numRegs);
+            return PB200_ERR_LAUNCH;
+        }
         attr_set.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
     }
     auto map = [&](CUtensorMap* m, const void* base, int64_t rows, uint32_t box_rows) {

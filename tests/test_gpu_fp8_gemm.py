@@ -114,7 +114,8 @@ def test_special_scales_and_values_stay_in_their_rows(M):
     assert torch.equal(out[keep.cuda()], clean[keep.cuda()])
 
 
-@pytest.mark.parametrize("M,N,K", [(8192, 264, 128), (4096, 520, 64), (16384, 136, 128), (4096, 4096, 128)])
+@pytest.mark.parametrize("M,N,K", [(8192, 264, 128), (4096, 520, 64), (16384, 136, 128), (4096, 4096, 128),
+                                   (40000, 120, 128)])
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_tiles_in_quick_succession(M, N, K, kind):
     """One scale block a tile and several tiles a CTA: a tile's results leave through buffers that the next
