@@ -569,9 +569,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   few rows (32 at most; 16 for each expert on average, since loads are uneven): 32 x 128 tiles.
 //   dense: 128 x 128 tiles while they fit the SMs at once (512 x 4096 x 4096: 13.4 us, as pairs 16.4), else
 //   256 x 256 tiles of CTA pairs (768 x 4096 x 4096: 17.7 us, as 128 x 128 ones one after the other 21.6),
-//   unless a pair's tile would be half empty (N <= 128).  Where 128-column tiles leave SMs idle the K blocks of
-//   a tile are shared by a cluster of up to 8 CTAs (at least eight blocks each: the cluster's two barriers
-//   take about 1.6 us), which add their partial tiles through distributed shared memory in a fixed order.
+//   unless a pair's tile would be half empty (40000 x 128 x 4096: 42 us, as pairs 50).  Where 128-column tiles
+//   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least eight blocks each:
+//   the cluster's two barriers take about 1.6 us), which add their partial tiles through distributed shared
+//   memory in a fixed order.
 //   grouped: the tiles are known on the device only, so the rows an expert has on average decide: pairs above
 //   128 (32 experts, 4096 x 2048: 128 rows 73 us on 128 x 128 tiles, 76 as pairs; 200 rows 96 and 91).
 struct Plan {

@@ -11,9 +11,8 @@
 // Launcher is the same launch with everything static bound to the kernel object: one call from
 // Python checks the inputs against the specs, takes the current stream, allocates and launches.
 // A call of ours costs the host about as long as a small kernel runs, so this path decides what a
-// chain of small calls costs (measured on the GPU host: DISPATCH_US_AFTER us a call against DISPATCH_US_BEFORE us with the checks in
-// Python).  It answers None for whatever it does not accept, and the caller takes the checking path,
-// which words the errors.
+// chain of small calls costs (measured: 4 to 5.5 us a call against 11.5 with the checks in Python).  It answers
+// None for whatever it does not accept, and the caller takes the checking path, which words the errors.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/cuda/EmptyTensor.h>
