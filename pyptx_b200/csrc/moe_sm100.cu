@@ -16,6 +16,8 @@
 #include "common.cuh"
 #include "ptx.cuh"
 
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -653,6 +655,9 @@ size_t route_smem(int64_t n, int64_t experts, int ctas) {
     return tables + (route_in_regs(n, ctas) ? (size_t)route_per_warp(n, ctas) * kRouteWarps * sizeof(int2) : 0);
 }
 
+constexpr int kRouteMaxSmem = (kRouteWarps + 5) * kMaxExperts * (int)sizeof(int) + 32 * kRouteRegSteps * kRouteWarps * (int)sizeof(int2);
+static_assert(kRouteMaxSmem + 2 * kRouteWarps * (int)sizeof(int) <= 227 * 1024, "shared memory of the route kernel");
+
 bool is_bf16(const Record& r) { return (r.flags & PB200_F_OUT_BF16) != 0; }
 
 // Steps of a warp (each `step` wide) over a row of `width`: the most, up to `most`, that still leave a few warps
@@ -687,8 +692,16 @@ int launch_route(const Record& r, cudaStream_t stream, void** p, char* err) {
     a.per_warp = (int)route_per_warp(n, ctas);
     auto kernel = route_in_regs(n, ctas) ? route_kernel<IdT, true> : route_kernel<IdT, false>;
     const size_t smem = route_smem(n, a.experts, ctas);
+    static std::atomic<uint64_t> attr_set[2];       // bit per device, for the two kernels of this id type
+    std::atomic<uint64_t>& done = attr_set[route_in_regs(n, ctas)];
     cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(done.load(std::memory_order_relaxed) & (1ull << (dev & 63)))) {
+        // The limit belongs to the kernel, not to a launch: one for all sizes, since another thread may launch another size.
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteMaxSmem);
+        if (e == cudaSuccess) done.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+    }
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(ctas);

@@ -102,6 +102,39 @@ def test_side_stream_and_threads():
             assert all(torch.equal(a, b) for a, b in zip(out, want[n]))
 
 
+def test_threads_that_route_different_sizes():
+    """Shared memory differs between these (one needs 217 KB, one 54 KB, one 164 KB); none may narrow another's limit."""
+    import threading
+
+    shapes = [(32768, 2, 1024), (2048, 1, 255), (16384, 1, 1000)]
+    routes = [moe.build_moe_route(T, k, E, block=1) for T, k, E in shapes]
+    ids = [torch.randint(0, E, (T, k), dtype=torch.int32, device="cuda") for T, k, E in shapes]
+    torch.cuda.synchronize()
+    errors, counts = [], [0] * len(shapes)
+    start = threading.Barrier(len(shapes))
+
+    def work(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()) as _:
+                start.wait()
+                for _ in range(300):
+                    row_of, entry_of, offsets = routes[n](ids[n])
+                torch.cuda.current_stream().synchronize()
+            order = torch.sort(ids[n].flatten(), stable=True).indices
+            assert torch.equal(entry_of.long(), order)
+            counts[n] += 1
+        except Exception as exc:  # noqa: BLE001
+            errors.append(exc)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(len(shapes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert counts == [1] * len(shapes)
+
+
 @pytest.mark.parametrize("kind", ["gemm", "fp8_gemm", "rms_norm"])
 def test_a_thread_whose_first_cuda_call_is_a_launch(kind):
     """The raw entry from a host thread that has made no CUDA call (and so has no context bound)."""
