@@ -30,6 +30,7 @@ constexpr int kMaxTopK = 32;                  // one lane holds one choice's row
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxBlock = 1024;
 constexpr int kScaleBlock = 128;
+constexpr int64_t kMaxExtent = 0x7fff0000;    // a step past the last row or column still fits 32 bits
 
 __device__ __forceinline__ void pdl_prologue() {
     ptx::pdl_launch_dependents();
@@ -762,7 +763,7 @@ int plan_moe(Record& r, char* err) {
     if (r.n_dims != need) { set_err(err, "kernel %d needs %d dims, got %d", r.kernel_id, need, r.n_dims); return PB200_ERR_BAD_SHAPE; }
     for (int i = 0; i < need; ++i) {
         if (r.dims[i] < 1) return bad("all sizes must be positive");
-        if (r.dims[i] > 0x7fffffffLL) return bad("extent exceeds 2^31-1");
+        if (r.dims[i] > kMaxExtent) return bad("extent exceeds 2^31-65536");
     }
     if (r.kernel_id == PB200_K_FP8_QUANTIZE) {
         const int64_t M = r.dims[0], K = r.dims[1];

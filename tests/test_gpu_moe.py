@@ -217,6 +217,21 @@ def test_quantize_is_exact(M, K, kind, block_rows):
 
 
 @pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_the_longest_row(block_rows):
+    """2^31 - 65536 columns, the most that is accepted."""
+    K = 2 ** 31 - 65536
+    x = torch.zeros(1, K, dtype=torch.bfloat16, device="cuda")
+    at = [5, 2 ** 30, K - 200, K - 1]
+    for i, c in enumerate(at):
+        x[0, c] = 448.0 * 2 ** i
+    q, scale = build_fp8_quantize(1, K, block_rows=block_rows)(x)
+    assert int(torch.count_nonzero(q.view(torch.uint8).view(torch.int32))) == len(at)
+    assert int((scale > 2.0 ** -100).sum()) == len(at)
+    for i, c in enumerate(at):
+        assert float(q[0, c]) == 448.0 and float(scale[0, c // 128]) == 2.0 ** i
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
 def test_quantize_special_blocks(block_rows):
     """All zeros, the smallest numbers, the largest, a NaN, an infinity: one 128-column block each."""
     M, K = 128, 128 * 6

@@ -93,6 +93,9 @@ def test_builders_refuse(call, message):
     (_ids.K_FP8_QUANTIZE, (4, 24, 1), "divisible by 16"),
     (_ids.K_FP8_QUANTIZE, (4, 32, 2), "block_rows"),
     (_ids.K_FP8_QUANTIZE, (2 ** 30, 2 ** 20, 1), "too large"),
+    (_ids.K_FP8_QUANTIZE, (1, 2 ** 31 - 16, 1), "exceeds"),
+    (_ids.K_MOE_ROUTE, (4, 2, 8, 1, 2 ** 31 - 4096), "exceeds"),
+    (_ids.K_MOE_DISPATCH_FP8, (1, 1, 1, 2 ** 31 - 16), "exceeds"),
 ])
 def test_library_refuses(kid, dims, message):
     rc, text = _create(kid, dims)
