@@ -13,15 +13,18 @@
 // What bounds it at large sizes: a CTA's 128 x 256 x 128 block takes 512 clocks of MMA, 512 of operands
 // from L2 (64 bytes a clock), and the drain of its accumulators 286 clocks of each SM sub-partition's
 // TMEM port and FMA pipe.  The three overlap, but the way MMA -> commit -> epilogue -> release -> MMA
-// has 390 clocks of latency besides the work, and TMEM holds two blocks: a block takes 720 clocks, plus
-// 2600 a tile for its store and the restart (8192 x 8192 x 4096: 229 us, 2400 TFLOP/s back to back, tensor
-// pipe 70 % active; 2040 when run for seconds, under the power cap).
+// is long, TMEM holds two blocks, and the instructions that issue a block's MMAs take nearly as long as the
+// MMAs: a block takes 690 clocks (630 with an epilogue that only hands accumulators back), plus 3000 a tile
+// for its store and the restart (1400 of them go without the writes themselves).  8192 x 8192 x 4096: 224 us,
+// 2450 TFLOP/s back to back; 2110 when run for seconds, under the power cap.
 // What brought it there (8192 x 8192 x 4096): pairs of CTAs with four accumulators of 128 columns instead of
 // two of 256, so that a half is released while the other runs; MMAs issued from uniform registers by an
 // elected lane (from a lane's own they issue at 60 clocks each); the next barriers looked at under the
 // current work, in the issuing warp and in the epilogue; scales copied into shared memory a group of
-// blocks ahead (read from global memory by the epilogue they cost 700 clocks a block): 345 -> 229 us.
-// Two issuing warps, and 16 epilogue warps with 64 columns each, measured slower.
+// blocks ahead (read from global memory by the epilogue they cost 700 clocks a block); fewer instructions
+// between one half's MMAs and the next, and accumulators handed back after two batches of loads: 345 -> 224 us.
+// Two issuing warps, 16 epilogue warps with 64 columns each, warps that take 64 columns of both halves, and
+// accumulators of 256 columns measured slower.
 //
 // Structure as the bf16 GEMM's (gemm_sm100.cu): persistent, one warp = TMA producer, one = MMA issuer and
 // TMEM owner, one copies scales, the epilogue's warps two for each quarter of the lanes, each with half of
@@ -60,8 +63,9 @@ constexpr int kPartPitch = 128 + 4;          // f32 row pitch of a split's parti
 static_assert(kSmemTotal <= 227 * 1024, "shared memory");
 constexpr int kMaxSplit = 8;
 // Registers of the 256-column form, whose epilogue threads hold 128 sums: the launch has 384 x 168;
-// the control warpgroup gives up 128 x 128 of them and the two epilogue warpgroups take 256 x 64.
-constexpr int kControlRegs = 40, kEpilogueRegs = 232;
+// the control warpgroup gives up 128 x 112 of them and the two epilogue warpgroups take 256 x 56 (with 16 a
+// thread more for these and as many less for the control warps, the control warps spill).
+constexpr int kControlRegs = 56, kEpilogueRegs = 224;
 static_assert(128 * kControlRegs + 256 * kEpilogueRegs <= kLaunchThreads * 168, "register split");     // checked at the first launch too
 
 // kind::f8f6f4 with e4m3 operands (format code 0) and f32 accumulation has the same fields as kind::f16.
@@ -302,22 +306,25 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const uint64_t da0 = make_desc_kmajor_sw128(s_ring), db0 = make_desc_kmajor_sw128(s_ring + kABytes);
             const uint32_t a_hi = (uint32_t)(da0 >> 32), b_hi = (uint32_t)(db0 >> 32);
             const bool leader = elect_one();
-            // The tensor pipe holds only a few MMAs, so a look at two barriers between blocks would drain it: the
-            // next barriers are looked at while this half's MMAs execute.
-            bool ok = true, full_seen = false, tempty_seen = false;
+            // The tensor pipe holds only a few MMAs, so that anything between one half's last and the next one's first
+            // drains it: the next barriers are looked at, and the lanes' answers joined, before this half's last MMA
+            // (a vote and two branches less between halves: 8192 x 8192 x 4096 194 -> 187 us on zeros).
+            bool ok = true, ready = false;
             for (int i = 0; i < total && ok; ++i) {
-                if (!full_seen) ok = mbar_wait(bar_full + 8 * stage, phase, ctx, 3);
                 const uint32_t a_lo = (uint32_t)da0 + (uint32_t)(stage * (kStage >> 4));
                 const uint32_t b_lo = (uint32_t)db0 + (uint32_t)(stage * (kStage >> 4));
-                const uint32_t empty = bar_empty + 8 * stage;
+                const uint32_t empty = bar_empty + 8 * stage, full = bar_full + 8 * stage, full_phase = phase;
                 if (++stage == kStages) { stage = 0; phase ^= 1u; }
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h) {
-                    if (ok && !tempty_seen) ok = mbar_wait(bar_tempty + 8 * acc, acc_phase ^ 1u, ctx, 2);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after_sync();
                     const uint32_t d = tmem_base + (uint32_t)(acc * kAccCols), tfull = bar_tfull + 8 * acc;
+                    if (!ready) {
+                        if (h == 0) ok = mbar_wait(full, full_phase, ctx, 3);
+                        if (ok) ok = mbar_wait(bar_tempty + 8 * acc, acc_phase ^ 1u, ctx, 2);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                    }
+                    tc_fence_after_sync();
                     const uint32_t b_half = b_lo + (uint32_t)(h * (kBRows * BK >> 4));
                     if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
                     // 32 e4m3 along K = 32 bytes = +2 in the encoded address
@@ -326,8 +333,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         umma_f8_ss<CTA_GROUP>(d, a_lo + 2, a_hi, b_half + 2, b_hi, kIdesc, 1u);
                         umma_f8_ss<CTA_GROUP>(d, a_lo + 4, a_hi, b_half + 4, b_hi, kIdesc, 1u);
                     }
-                    tempty_seen = mbar_test_wait(bar_tempty + 8 * acc, acc_phase ^ 1u);
-                    if (h == kHalves - 1) full_seen = mbar_test_wait(bar_full + 8 * stage, phase);
+                    ready = mbar_test_wait(bar_tempty + 8 * acc, acc_phase ^ 1u);
+                    if (h == kHalves - 1) ready = mbar_test_wait(bar_full + 8 * stage, phase) && ready;
+                    ready = __all_sync(0xffffffffu, ready);
                     if (leader) {
                         umma_f8_ss<CTA_GROUP>(d, a_lo + 6, a_hi, b_half + 6, b_hi, kIdesc, 1u);
                         if (CTA_GROUP == 2) umma_commit_pair(tfull); else umma_commit<1>(tfull);
@@ -335,9 +343,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                             if (CTA_GROUP == 2) umma_commit_pair(empty); else umma_commit<1>(empty);
                         }
                     }
-                    __syncwarp();
                 }
             }
+            __syncwarp();
         }
         if (warp == 3) {
             // Scales: this warp copies a group of blocks ahead into shared memory (four rows a lane), so that
@@ -411,16 +419,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     }
                     tc_fence_after_sync();
                     const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kAccCols + col_in_acc);
+                    // The accumulator is handed back once its last columns are in registers: two batches of loads
+                    // (tcgen05.wait::ld waits for all that are in flight), the second under the FMAs of the first.
                     constexpr int kChunks = kCols / 32;
-                    uint32_t v[2][32];                       // the next 32 columns arrive under the FMAs
+                    static_assert(kChunks == 2 || kChunks == 4, "two batches");
+                    uint32_t v[2][32];
                     tmem_ld_32x32b_x32(t_row, v[0]);
+                    tmem_ld_32x32b_x32(t_row + 32, v[1]);
+                    tmem_ld_wait();
+                    reg_fence(v[0]);
+                    reg_fence(v[1]);
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
-                        tmem_ld_wait();
-                        reg_fence(v[c & 1]);
-                        if (c + 1 < kChunks) {
-                            tmem_ld_32x32b_x32(t_row + (c + 1) * 32, v[(c + 1) & 1]);
-                        } else {
+                        if (c == kChunks - 2) {
+                            if (kChunks > 2) { tmem_ld_wait(); reg_fence(v[0]); reg_fence(v[1]); }
                             tc_fence_before_sync();
                             __syncwarp();
                             if (lane == 0) {
@@ -428,14 +440,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                                 else mbar_arrive(bar_tempty + 8 * acc);
                             }
                             if ((acc += kAccStep) >= kAccs) { acc = acc0; acc_phase ^= 1u; }
-                            seen = mbar_test_wait(bar_tfull + 8 * acc, acc_phase);
                             const int next = min(i + 1, n_blocks - 1);
                             s_next = sa[next * BM] * sb[next];
                         }
+                        if (c == kChunks - 1) seen = mbar_test_wait(bar_tfull + 8 * acc, acc_phase);
 #pragma unroll
                         for (int j = 0; j < 32; j += 2)
                             fma2v(sum[c * 32 + j], sum[c * 32 + j + 1], __uint_as_float(v[c & 1][j]), __uint_as_float(v[c & 1][j + 1]),
                                   s, s, sum[c * 32 + j], sum[c * 32 + j + 1]);
+                        if (c + 2 < kChunks) {
+                            reg_fence(v[c & 1]);
+                            tmem_ld_32x32b_x32(t_row + (c + 2) * 32, v[c & 1]);
+                        }
                     }
                 }
                 if (kb + kGroup >= kb1) break;               // the tile's last group is handed back below
