@@ -585,18 +585,21 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tile shape and split of K.
-//   8 rows at most, dense: the streaming kernel of fp8_gemm_skinny.cu (1 x 4096 x 4096 from HBM: 5.4 us against
-//   7.4 on 32 x 128 tiles), with 9 to 16 rows up to 16 Mi weights, since its arithmetic doubles (16 x 4096 x 4096:
-//   6.6 against 7.8 us, but 16 x 8192 x 8192: 19.5 against 15).
-//   few rows (32 at most; 16 for each expert on average, since loads are uneven): 32 x 128 tiles.
-//   dense: 128 x 128 tiles while they fit the SMs at once (512 x 4096 x 4096: 13.4 us, as pairs 16.4), else
-//   256 x 256 tiles of CTA pairs (768 x 4096 x 4096: 17.7 us, as 128 x 128 ones one after the other 21.6),
+//   8 rows at most, dense: the streaming kernel of fp8_gemm_skinny.cu (1 x 4096 x 4096 from HBM: 5.5 us against
+//   7.0 on 32 x 128 tiles), with 9 to 16 rows up to 16 Mi weights, since its arithmetic doubles (16 x 4096 x 4096:
+//   6.7 against 7.4 us, but 16 x 8192 x 8192: 19.5 against 15).
+//   few rows: 32 x 128 tiles; dense up to 32 rows (32 x 4096 x 4096: 7.5 us, on 128 x 128 tiles 7.7), grouped up to 24
+//   for each expert on average, since loads are uneven (32 experts, 4096 x 2048: 24 rows 48.6 us, on 128 x 128 tiles
+//   52.3; 28 rows 54.5 and 52.8).
+//   dense: 128 x 128 tiles while they fit the SMs at once (512 x 4096 x 4096: 11.6 us, as pairs 16.2), else
+//   256 x 256 tiles of CTA pairs (768 x 4096 x 4096: 17.0 us, as 128 x 128 ones one after the other 21.3),
 //   unless a pair's tile would be half empty (40000 x 128 x 4096: 42 us, as pairs 50).  Where 128-column tiles
 //   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least eight blocks each:
 //   the cluster's two barriers take about 1.6 us), which add their partial tiles through distributed shared
 //   memory in a fixed order.
-//   grouped: the tiles are known on the device only, so the rows an expert has on average decide: pairs above
-//   128 (32 experts, 4096 x 2048: 128 rows 73 us on 128 x 128 tiles, 76 as pairs; 200 rows 96 and 91).
+//   grouped: the tiles are known on the device only, so the rows an expert has on average decide: pairs from
+//   128 (32 experts, 4096 x 2048: 96 rows 60 us on 128 x 128 tiles, 71 as pairs; 128 rows 74.7 and 72.2; 200 rows
+//   92 and 75).
 struct Plan {
     int64_t experts, m, n, k, tiles;
     int bn, rows, split;
@@ -617,8 +620,8 @@ Plan make_plan(const Record& r) {
         p.tiles = fp8_skinny_grid(p.n);
         return p;
     }
-    if (mean_rows <= (grouped ? kSmallRows / 2 : kSmallRows)) { p.bn = 128; p.rows = kSmallRows; }
-    else if (p.n > 128 && (grouped ? mean_rows > 128 : ceil_div(p.m, BM) * ceil_div(p.n, 128) > sms)) { p.bn = 256; p.rows = BM; }
+    if (mean_rows <= (grouped ? kSmallRows * 3 / 4 : kSmallRows)) { p.bn = 128; p.rows = kSmallRows; }
+    else if (p.n > 128 && (grouped ? mean_rows >= BM : ceil_div(p.m, BM) * ceil_div(p.n, 128) > sms)) { p.bn = 256; p.rows = BM; }
     else { p.bn = 128; p.rows = BM; }
     // every expert may end in a partial tile
     p.tiles = (ceil_div(p.m, p.rows * p.cta_group()) + p.experts) * ceil_div(p.n, p.bn);

@@ -182,7 +182,7 @@ def _grouped(counts, N, K, kind, capacity=None, first=0):
 @pytest.mark.parametrize("counts,N,K", [
     ([1], 8, 16), ([0, 1, 0], 128, 128), ([5, 0, 0, 7, 1], 264, 272), ([128, 128], 256, 256), ([130, 1, 33, 32, 300], 520, 640),
     ([0] * 63 + [3], 136, 144), ([2] * 300, 72, 128), ([1000, 0, 17], 1032, 528), ([40, 700, 3, 260], 384, 1024),
-    ([1] * 1024, 64, 64), ([513, 255, 256, 1, 0, 700], 264, 272), ([300, 2500], 520, 1296),
+    ([1] * 1024, 64, 64), ([24, 40, 8, 24], 264, 1168), ([100, 27, 0, 90], 384, 1552), ([513, 255, 256, 1, 0, 700], 264, 272), ([300, 2500], 520, 1296),
 ])
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 def test_grouped(counts, N, K, kind):
@@ -190,9 +190,9 @@ def test_grouped(counts, N, K, kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
-@pytest.mark.parametrize("counts,N,K", [([128] * 40, 1024, 128), ([96, 32, 128] * 20, 640, 64), ([700, 300] * 4, 2048, 128)])
+@pytest.mark.parametrize("counts,N,K", [([128] * 40, 1024, 128), ([120] * 40, 1024, 128), ([24] * 100, 640, 1040), ([96, 32, 128] * 20, 640, 64), ([700, 300] * 4, 2048, 128)])
 def test_grouped_tiles_in_quick_succession(counts, N, K, kind):
-    """As above for the grouped forms: 128-column tiles (128 rows an expert and fewer) and CTA pairs."""
+    """As above for the grouped forms: 128-column tiles (fewer than 128 rows an expert) and CTA pairs."""
     for _ in range(3):
         _grouped(counts, N, K, kind)
 
