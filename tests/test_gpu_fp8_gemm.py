@@ -163,6 +163,35 @@ def test_repeated_calls_give_the_same_bits():
             assert torch.equal(kernel(a, sa, b, sb), first)
 
 
+@pytest.mark.parametrize("M", [1, 12, 40])
+def test_a_weight_made_by_the_kernel_before(M):
+    """The weight is quantised right before each product, replay after replay: no stale bytes."""
+    N, K = 1024, 4096
+    quantize, gemm = build_fp8_quantize(N, K, block_rows=128), build_fp8_gemm(M, N, K)
+    w = torch.empty(N, K, dtype=torch.bfloat16, device="cuda")
+    a, sa = torch.randn(M, K, device="cuda").to(torch.float8_e4m3fn), torch.rand(M, K // 128, device="cuda")
+    gemm(a, sa, *quantize(w.zero_()))
+    graph, outs = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(graph):
+        for _ in range(8):                       # the same buffers again and again, another weight each time
+            q, s = quantize(w)
+            outs.append(gemm(a, sa, q, s))
+            del q, s
+            w.neg_().mul_(1.5)
+    for seed in range(5):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        w.normal_(generator=g)
+        graph.replay()
+        got = [o.clone() for o in outs]
+        w.normal_(generator=g.manual_seed(seed))
+        for o in got:
+            torch.cuda.synchronize()
+            q, s = quantize(w)
+            torch.cuda.synchronize()
+            assert torch.equal(o, gemm(a, sa, q, s))
+            w.neg_().mul_(1.5)
+
+
 # ---- grouped ------------------------------------------------------------------------------------
 
 def _grouped(counts, N, K, kind, capacity=None, first=0):
