@@ -585,9 +585,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tile shape and split of K.
-//   8 rows at most, dense: the streaming kernel of fp8_gemm_skinny.cu (1 x 4096 x 4096 from HBM: 5.5 us against
+//   8 rows at most, dense: the streaming kernel of fp8_gemm_skinny.cu (1 x 4096 x 4096 from HBM: 4.9 us against
 //   7.0 on 32 x 128 tiles), with 9 to 16 rows up to 16 Mi weights, since its arithmetic doubles (16 x 4096 x 4096:
-//   6.7 against 7.4 us, but 16 x 8192 x 8192: 19.5 against 15).
+//   6.4 against 7.4 us, but 16 x 8192 x 8192: 19.5 against 15).
 //   few rows: 32 x 128 tiles; dense up to 32 rows (32 x 4096 x 4096: 7.5 us, on 128 x 128 tiles 7.7), grouped up to 24
 //   for each expert on average, since loads are uneven (32 experts, 4096 x 2048: 24 rows 48.6 us, on 128 x 128 tiles
 //   52.3; 28 rows 54.5 and 52.8).
