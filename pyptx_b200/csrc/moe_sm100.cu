@@ -94,10 +94,13 @@ template <> struct Vec<__nv_bfloat16> {
 // in the same launch, so nothing has to be cleared beforehand.
 //
 // Latency-bound: the ids are read once (4 or 8 bytes an entry), the maps written once.  In a chain of
-// graph launches 128 entries take 4.0 us, 32768 (eight CTAs, 32 experts) 7.2 us.
+// graph launches 128 entries take 3.5 us, 32768 (eight CTAs, 32 experts) 7.1 us.
 // ---------------------------------------------------------------------------
-constexpr int kRouteThreads = 1024;
-constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteThreads = 1024;           // of a CTA; kRouteFewThreads for few entries and experts
+constexpr int kRouteFewThreads = 256;
+constexpr int kRouteFewEntries = 512, kRouteFewExperts = 128;
+static_assert(kRouteFewEntries <= kRouteFewThreads * 8, "few entries stay in registers");
+static_assert(kRouteFewExperts <= kRouteFewThreads, "a thread for each expert");
 constexpr int kRouteMaxCtas = 8;
 constexpr int kMaxIdBits = 10;                // ids below kMaxExperts
 static_assert(1 << kMaxIdBits >= kMaxExperts, "id bits");
@@ -144,26 +147,27 @@ __device__ __forceinline__ int warp_rank(int* counters, int id, int lane, int id
     return base + __popc(before);
 }
 
-template <typename IdT, bool IN_REGS>
-__global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
+template <typename IdT, int THREADS, bool IN_REGS>
+__global__ void __launch_bounds__(THREADS, 1) route_kernel(RouteArgs a) {
+    constexpr int kWarpsHere = THREADS / 32;
     pdl_prologue();
     extern __shared__ int smem[];
     const int E = a.experts;
     int* counters = smem;                           // [warps][E]: counts, then prefix over warps
-    int* cta_count = counters + kRouteWarps * E;    // [E], read by the other CTAs
+    int* cta_count = counters + kWarpsHere * E;    // [E], read by the other CTAs
     int* base = cta_count + E;                      // [E] first row of this CTA's entries of an expert
     int* filled = base + E;                         // [E] end of the expert's entries (row)
     int* ends = filled + E;                         // [E] end of the expert's rows
     int* local = ends + E;                          // [E] first place of an expert among this CTA's sorted entries
     int2* sorted = reinterpret_cast<int2*>(local + E + (E & 1));      // IN_REGS: (row, entry) of this CTA's entries, by expert
-    __shared__ int warp_total[kRouteWarps], warp_own[kRouteWarps];
+    __shared__ int warp_total[32], warp_own[32];
 
     uint32_t n_ctas;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n_ctas));
     const int rank = (int)ptx::cluster_ctarank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int id_bits = 32 - __clz(E - 1);          // E = 1: none
-    const int first = (rank * kRouteWarps + warp) * a.per_warp;
+    const int first = (rank * kWarpsHere + warp) * a.per_warp;
     const int steps = first < a.n ? (min(a.per_warp, a.n - first) + 31) / 32 : 0;
 
     int my_id[kRouteRegSteps], my_rank[kRouteRegSteps];
@@ -171,7 +175,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
 #pragma unroll
         for (int r = 0; r < kRouteRegSteps; ++r) my_id[r] = r < steps ? load_id<IdT>(a.ids, first + r * 32 + lane, a.n, E) : -1;
     }
-    for (int i = tid; i < kRouteWarps * E; i += kRouteThreads) counters[i] = 0;
+    for (int i = tid; i < kWarpsHere * E; i += THREADS) counters[i] = 0;
     __syncthreads();
     if (IN_REGS) {
 #pragma unroll
@@ -188,10 +192,10 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     }
     __syncthreads();
     // prefix over warps: counters[w][e] = entries of e in earlier warps of this CTA
-    for (int e = tid; e < E; e += kRouteThreads) {
+    for (int e = tid; e < E; e += THREADS) {
         int run = 0;
 #pragma unroll 8
-        for (int w = 0; w < kRouteWarps; ++w) {
+        for (int w = 0; w < kWarpsHere; ++w) {
             const int c = counters[w * E + e];
             counters[w * E + e] = run;
             run += c;
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
         cta_count[e] = run;
     }
     if (n_ctas > 1) ptx::cluster_sync_all(); else __syncthreads();
-    // totals over CTAs, then a block-wide exclusive prefix of the padded totals (E <= 1024 threads)
+    // totals over CTAs, then a block-wide exclusive prefix of the padded totals (E <= THREADS)
     int total = 0, before = 0, own_count = 0;
     if (tid < E) {
         own_count = cta_count[tid];
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
     __syncthreads();
     if (warp < 2) {
         int* totals = warp == 0 ? warp_total : warp_own;
-        int v = totals[lane];
+        int v = lane < kWarpsHere ? totals[lane] : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
             }
         }
         __syncthreads();
-        for (int k = tid; k < warp_own[kRouteWarps - 1]; k += kRouteThreads) {
+        for (int k = tid; k < warp_own[kWarpsHere - 1]; k += THREADS) {
             const int2 at = sorted[k];
             if (at.x >= 0) a.entry_of[at.x] = at.y;
         }
@@ -289,9 +293,9 @@ __global__ void __launch_bounds__(kRouteThreads, 1) route_kernel(RouteArgs a) {
         }
     }
     // rows without an entry: each expert's padding, then everything behind the last expert
-    for (int e = rank * kRouteWarps + warp; e < E; e += (int)n_ctas * kRouteWarps)
+    for (int e = rank * kWarpsHere + warp; e < E; e += (int)n_ctas * kWarpsHere)
         for (int r = filled[e] + lane; r < min(ends[e], a.rows); r += 32) a.entry_of[r] = -1;
-    for (int r = ends[E - 1] + rank * kRouteThreads + tid; r < a.rows; r += (int)n_ctas * kRouteThreads) a.entry_of[r] = -1;
+    for (int r = ends[E - 1] + rank * THREADS + tid; r < a.rows; r += (int)n_ctas * THREADS) a.entry_of[r] = -1;
     if (n_ctas > 1) ptx::cluster_wait();            // shared memory must outlive the other CTAs' reads
 }
 
@@ -642,6 +646,12 @@ __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(MoveArgs a) {
 // ---------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Threads of a CTA: few entries and experts are sorted sooner by few warps, which meet at every barrier (graph
+// replay: 16 entries over 8 experts 2.8 us, with 1024 threads 3.9; 512 over 64 3.7 and 4.0; but 256 over 256 8.2 and
+// 6.4, 1024 over 32 4.7 and 4.6).
+int route_threads(int64_t n, int64_t experts) {
+    return n <= kRouteFewEntries && experts <= kRouteFewExperts ? kRouteFewThreads : kRouteThreads;
+}
 int route_ctas(int64_t n) {
     // One CTA ranks 32 entries a warp and step; a second CTA costs a cluster barrier, so the cluster
     // grows only once a CTA would walk more than two steps.
@@ -649,15 +659,16 @@ int route_ctas(int64_t n) {
     while (ctas < kRouteMaxCtas && n > (int64_t)ctas * 2 * kRouteThreads) ctas *= 2;
     return ctas;
 }
-int64_t route_per_warp(int64_t n, int ctas) { return ceil_div(ceil_div(n, ctas * kRouteWarps), 32) * 32; }
-bool route_in_regs(int64_t n, int ctas) { return route_per_warp(n, ctas) <= 32 * kRouteRegSteps; }
-size_t route_smem(int64_t n, int64_t experts, int ctas) {
-    const size_t tables = ((size_t)(kRouteWarps + 5) * experts + (experts & 1)) * sizeof(int);
-    return tables + (route_in_regs(n, ctas) ? (size_t)route_per_warp(n, ctas) * kRouteWarps * sizeof(int2) : 0);
+int64_t route_per_warp(int64_t n, int ctas, int threads) { return ceil_div(ceil_div(n, ctas * (threads / 32)), 32) * 32; }
+bool route_in_regs(int64_t per_warp) { return per_warp <= 32 * kRouteRegSteps; }
+size_t route_smem(int64_t n, int64_t experts) {
+    const int ctas = route_ctas(n), threads = route_threads(n, experts), warps = threads / 32;
+    const int64_t per_warp = route_per_warp(n, ctas, threads);
+    const size_t tables = ((size_t)(warps + 5) * experts + (experts & 1)) * sizeof(int);
+    return tables + (route_in_regs(per_warp) ? (size_t)per_warp * warps * sizeof(int2) : 0);
 }
-
-constexpr int kRouteMaxSmem = (kRouteWarps + 5) * kMaxExperts * (int)sizeof(int) + 32 * kRouteRegSteps * kRouteWarps * (int)sizeof(int2);
-static_assert(kRouteMaxSmem + 2 * kRouteWarps * (int)sizeof(int) <= 227 * 1024, "shared memory of the route kernel");
+constexpr int kRouteMaxSmem = (kRouteThreads / 32 + 5) * kMaxExperts * (int)sizeof(int) + kRouteThreads * kRouteRegSteps * (int)sizeof(int2);
+static_assert(kRouteMaxSmem + 64 * (int)sizeof(int) <= 227 * 1024, "shared memory of the route kernel");
 
 bool is_bf16(const Record& r) { return (r.flags & PB200_F_OUT_BF16) != 0; }
 
@@ -689,24 +700,25 @@ int launch_route(const Record& r, cudaStream_t stream, void** p, char* err) {
     a.experts = (int)r.dims[2];
     a.block = (int)r.dims[3];
     a.rows = (int)r.dims[4];
-    const int ctas = (int)r.geom.cluster[0];
-    a.per_warp = (int)route_per_warp(n, ctas);
-    auto kernel = route_in_regs(n, ctas) ? route_kernel<IdT, true> : route_kernel<IdT, false>;
-    const size_t smem = route_smem(n, a.experts, ctas);
-    static std::atomic<uint64_t> attr_set[2];       // bit per device, for the two kernels of this id type
-    std::atomic<uint64_t>& done = attr_set[route_in_regs(n, ctas)];
+    const int ctas = (int)r.geom.cluster[0], threads = (int)r.geom.block[0];
+    a.per_warp = (int)route_per_warp(n, ctas, threads);
+    const int form = threads == kRouteFewThreads ? 0 : route_in_regs(a.per_warp) ? 1 : 2;
+    auto kernel = form == 0 ? route_kernel<IdT, kRouteFewThreads, true>
+                : form == 1 ? route_kernel<IdT, kRouteThreads, true> : route_kernel<IdT, kRouteThreads, false>;
+    const size_t smem = route_smem(n, a.experts);
+    static std::atomic<uint64_t> attr_set[3];       // bit per device, for the kernels of this id type
     cudaError_t e = cudaSuccess;
     int dev = 0;
     cudaGetDevice(&dev);
-    if (!(done.load(std::memory_order_relaxed) & (1ull << (dev & 63)))) {
+    if (!(attr_set[form].load(std::memory_order_relaxed) & (1ull << (dev & 63)))) {
         // The limit belongs to the kernel, not to a launch: one for all sizes, since another thread may launch another size.
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteMaxSmem);
-        if (e == cudaSuccess) done.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+        if (e == cudaSuccess) attr_set[form].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
     }
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(ctas);
-        cfg.blockDim = dim3(kRouteThreads);
+        cfg.blockDim = dim3(threads);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = stream;
         cudaLaunchAttribute attr[2];
@@ -786,8 +798,8 @@ int plan_moe(Record& r, char* err) {
         if (block > kMaxBlock) { set_err(err, "block=%lld exceeds %d", (long long)block, kMaxBlock); return PB200_ERR_BAD_SHAPE; }
         if (rows % block != 0) { set_err(err, "rows=%lld must be divisible by block=%lld", (long long)rows, (long long)block); return PB200_ERR_BAD_SHAPE; }
         g.cluster[0] = g.grid[0] = (uint32_t)route_ctas(T * k);
-        g.block[0] = kRouteThreads;
-        g.smem_bytes = (uint32_t)route_smem(T * k, E, route_ctas(T * k));
+        g.block[0] = (uint32_t)route_threads(T * k, E);
+        g.smem_bytes = (uint32_t)route_smem(T * k, E);
         g.n_inputs = 1;
         g.n_outputs = 3;
         return PB200_OK;

@@ -41,7 +41,8 @@ def test_moe_rows_holds_every_outcome(T, k, E, block):
 def test_specs_and_geometry():
     route = moe.build_moe_route(64, 4, 16, block=16, ids_dtype=s64)
     assert route.in_specs[0].dtype is s64 and [s.shape for s in route.out_specs] == [(64, 4), (route.meta["rows"],), (17,)]
-    assert route.grid == (1, 1, 1) and route.block == (1024, 1, 1)
+    assert route.grid == (1, 1, 1) and route.block == (256, 1, 1)
+    assert moe.build_moe_route(64, 4, 256).block == moe.build_moe_route(1024, 4, 16).block == (1024, 1, 1)
     assert moe.build_moe_route(8192, 8, 64).cluster == (8, 1, 1)
     d = moe.build_moe_dispatch_fp8(64, 4, 256, 272)
     assert d.out_specs[0].dtype is e4m3 and d.out_specs[1].shape == (256, 3)
