@@ -164,7 +164,7 @@ extern "C" {
  *       buffers: ids[T,top_k] s32 (s64) -> row_of[T,top_k], entry_of[R], offsets[E+1] s32
  *       Entries sorted by expert, equal experts in entry order, each expert's rows padded to a multiple
  *       of block.  Entries whose id lies outside [0, E), or whose row would be R or above, get row -1;
- *       rows without an entry get entry -1; offsets are clipped to R.
+ *       rows without an entry get entry -1; offsets are clipped to R.  Above 32768 entries: + scratch, as above.
  *   PB200_K_MOE_DISPATCH      dims = {T, top_k, R, H}
  *       buffers: x[T,H], row_of, entry_of -> rows[R,H] (zeros where entry_of < 0)
  *   PB200_K_MOE_DISPATCH_FP8  dims = {T, top_k, R, H}          flags: PB200_F_IN_BF16

@@ -82,7 +82,7 @@ template <> struct Vec<__nv_bfloat16> {
 };
 
 // ---------------------------------------------------------------------------
-// Route: a stable counting sort in one launch of one cluster.
+// Route: a stable counting sort in one launch of one cluster (up to 32768 entries; see below for more).
 //
 // Entry i = t*k + j asks for expert ids[i].  CTA c of the cluster owns a contiguous range of
 // entries and each of its warps a contiguous part of that, so "earlier entry" is "earlier step of
@@ -94,17 +94,18 @@ template <> struct Vec<__nv_bfloat16> {
 // in the same launch, so nothing has to be cleared beforehand.
 //
 // Latency-bound: the ids are read once (4 or 8 bytes an entry), the maps written once.  In a chain of
-// graph launches 128 entries take 3.5 us, 32768 (eight CTAs, 32 experts) 7.1 us.
+// graph launches 128 entries take 3.2 us, 32768 (eight CTAs, 32 experts) 6.5 us.
 // ---------------------------------------------------------------------------
 constexpr int kRouteThreads = 1024;           // of a CTA; kRouteFewThreads for few entries and experts
 constexpr int kRouteFewThreads = 256;
-constexpr int kRouteFewEntries = 512, kRouteFewExperts = 128;
-static_assert(kRouteFewEntries <= kRouteFewThreads * 8, "few entries stay in registers");
-static_assert(kRouteFewExperts <= kRouteFewThreads, "a thread for each expert");
+constexpr int kRouteFewEntries = 256, kRouteFewExperts = 128;
 constexpr int kRouteMaxCtas = 8;
 constexpr int kMaxIdBits = 10;                // ids below kMaxExperts
 static_assert(1 << kMaxIdBits >= kMaxExperts, "id bits");
-constexpr int kRouteRegSteps = 8;            // steps whose ids and ranks stay in registers
+constexpr int kRouteRegSteps = 4;            // steps of a warp, whose ids and ranks stay in registers
+constexpr int64_t kRouteClusterEntries = (int64_t)kRouteMaxCtas * kRouteThreads * kRouteRegSteps;      // more take two launches
+static_assert(kRouteFewEntries <= kRouteFewThreads * kRouteRegSteps, "few entries stay in registers");
+static_assert(kRouteFewExperts <= kRouteFewThreads, "a thread for each expert");
 
 struct RouteArgs {
     const void* ids;
@@ -147,7 +148,7 @@ __device__ __forceinline__ int warp_rank(int* counters, int id, int lane, int id
     return base + __popc(before);
 }
 
-template <typename IdT, int THREADS, bool IN_REGS>
+template <typename IdT, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) route_kernel(RouteArgs a) {
     constexpr int kWarpsHere = THREADS / 32;
     pdl_prologue();
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(THREADS, 1) route_kernel(RouteArgs a) {
     int* filled = base + E;                         // [E] end of the expert's entries (row)
     int* ends = filled + E;                         // [E] end of the expert's rows
     int* local = ends + E;                          // [E] first place of an expert among this CTA's sorted entries
-    int2* sorted = reinterpret_cast<int2*>(local + E + (E & 1));      // IN_REGS: (row, entry) of this CTA's entries, by expert
+    int2* sorted = reinterpret_cast<int2*>(local + E + (E & 1));      // (row, entry) of this CTA's entries, by expert
     __shared__ int warp_total[32], warp_own[32];
 
     uint32_t n_ctas;
@@ -171,25 +172,13 @@ __global__ void __launch_bounds__(THREADS, 1) route_kernel(RouteArgs a) {
     const int steps = first < a.n ? (min(a.per_warp, a.n - first) + 31) / 32 : 0;
 
     int my_id[kRouteRegSteps], my_rank[kRouteRegSteps];
-    if (IN_REGS) {
 #pragma unroll
-        for (int r = 0; r < kRouteRegSteps; ++r) my_id[r] = r < steps ? load_id<IdT>(a.ids, first + r * 32 + lane, a.n, E) : -1;
-    }
+    for (int r = 0; r < kRouteRegSteps; ++r) my_id[r] = r < steps ? load_id<IdT>(a.ids, first + r * 32 + lane, a.n, E) : -1;
     for (int i = tid; i < kWarpsHere * E; i += THREADS) counters[i] = 0;
     __syncthreads();
-    if (IN_REGS) {
 #pragma unroll
-        for (int r = 0; r < kRouteRegSteps; ++r)
-            if (r < steps) my_rank[r] = warp_rank(counters + warp * E, my_id[r], lane, id_bits);
-    } else {
-        int next = load_id<IdT>(a.ids, first + lane, steps > 0 ? a.n : 0, E);
-        for (int r = 0; r < steps; ++r) {
-            const int i = first + r * 32 + lane, id = next;
-            next = r + 1 < steps ? load_id<IdT>(a.ids, i + 32, a.n, E) : -1;
-            const int rk = warp_rank(counters + warp * E, id, lane, id_bits);
-            if (i < a.n) a.row_of[i] = rk;          // kept for the second pass of this same thread
-        }
-    }
+    for (int r = 0; r < kRouteRegSteps; ++r)
+        if (r < steps) my_rank[r] = warp_rank(counters + warp * E, my_id[r], lane, id_bits);
     __syncthreads();
     // prefix over warps: counters[w][e] = entries of e in earlier warps of this CTA
     for (int e = tid; e < E; e += THREADS) {
@@ -256,47 +245,159 @@ __global__ void __launch_bounds__(THREADS, 1) route_kernel(RouteArgs a) {
         }
     }
     __syncthreads();
-    if (IN_REGS) {
-        // Entries go to entry_of by way of shared memory, sorted, so that neighbouring lanes store neighbouring
-        // rows (stored straight from the lanes they cost a sector each, and eight SMs store one a clock).
+    // Entries go to entry_of by way of shared memory, sorted, so that neighbouring lanes store neighbouring
+    // rows (stored straight from the lanes they cost a sector each, and eight SMs store one a clock).
 #pragma unroll
-        for (int r = 0; r < kRouteRegSteps; ++r) {
-            const int i = first + r * 32 + lane, id = my_id[r];
-            if (r < steps && i < a.n) {
-                int row = -1;
-                if (id >= 0) {
-                    const int k = counters[warp * E + id] + my_rank[r];
-                    row = base[id] + k;
-                    if (row >= a.rows) row = -1;                        // no room: dropped
-                    sorted[local[id] + k] = make_int2(row, i);
-                }
-                a.row_of[i] = row;
-            }
-        }
-        __syncthreads();
-        for (int k = tid; k < warp_own[kWarpsHere - 1]; k += THREADS) {
-            const int2 at = sorted[k];
-            if (at.x >= 0) a.entry_of[at.x] = at.y;
-        }
-    } else {
-#pragma unroll 4
-        for (int r = 0; r < steps; ++r) {
-            const int i = first + r * 32 + lane;
-            if (i >= a.n) continue;
-            const int id = load_id<IdT>(a.ids, i, a.n, E);
+    for (int r = 0; r < kRouteRegSteps; ++r) {
+        const int i = first + r * 32 + lane, id = my_id[r];
+        if (r < steps && i < a.n) {
             int row = -1;
             if (id >= 0) {
-                row = base[id] + counters[warp * E + id] + a.row_of[i];
-                if (row < a.rows) a.entry_of[row] = i; else row = -1;
+                const int k = counters[warp * E + id] + my_rank[r];
+                row = base[id] + k;
+                if (row >= a.rows) row = -1;                        // no room: dropped
+                sorted[local[id] + k] = make_int2(row, i);
             }
             a.row_of[i] = row;
         }
+    }
+    __syncthreads();
+    for (int k = tid; k < warp_own[kWarpsHere - 1]; k += THREADS) {
+        const int2 at = sorted[k];
+        if (at.x >= 0) a.entry_of[at.x] = at.y;
     }
     // rows without an entry: each expert's padding, then everything behind the last expert
     for (int e = rank * kWarpsHere + warp; e < E; e += (int)n_ctas * kWarpsHere)
         for (int r = filled[e] + lane; r < min(ends[e], a.rows); r += 32) a.entry_of[r] = -1;
     for (int r = ends[E - 1] + rank * THREADS + tid; r < a.rows; r += (int)n_ctas * THREADS) a.entry_of[r] = -1;
     if (n_ctas > 1) ptx::cluster_wait();            // shared memory must outlive the other CTAs' reads
+}
+
+// The same sort for more entries than a cluster's registers hold, on all SMs in two launches.  The first
+// ranks: row_of takes an entry's rank among its expert's entries of this CTA, counts[e][c] their number.  The
+// second adds what earlier CTAs and experts have (a warp sums an expert's counts, lanes along the CTAs) and places.
+// 65536 entries over 32 experts 6.5 us (on one cluster of eight CTAs 10.1), 524288 over 256 19 (96); at 32768 the
+// cluster is as quick (6.5 against 6.9 over 32 experts, 8.2 against 8.9 over 256) and takes one launch.
+template <typename IdT>
+__global__ void __launch_bounds__(kRouteThreads, 1) route_rank_kernel(RouteArgs a, int* counts) {
+    pdl_prologue();
+    extern __shared__ int counters[];               // [warps][E]: counts, then prefix over warps
+    constexpr int kWarpsHere = kRouteThreads / 32;
+    const int E = a.experts, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int id_bits = 32 - __clz(E - 1);
+    const int first = ((int)blockIdx.x * kWarpsHere + warp) * a.per_warp;
+    const int steps = first < a.n ? (min(a.per_warp, a.n - first) + 31) / 32 : 0;
+    for (int i = tid; i < kWarpsHere * E; i += kRouteThreads) counters[i] = 0;
+    __syncthreads();
+    int next = load_id<IdT>(a.ids, first + lane, steps > 0 ? a.n : 0, E);
+    for (int r = 0; r < steps; ++r) {
+        const int i = first + r * 32 + lane, id = next;
+        next = r + 1 < steps ? load_id<IdT>(a.ids, i + 32, a.n, E) : -1;
+        const int rk = warp_rank(counters + warp * E, id, lane, id_bits);
+        if (i < a.n) a.row_of[i] = rk;              // kept for the pass below of this same thread
+    }
+    __syncthreads();
+    for (int e = tid; e < E; e += kRouteThreads) {
+        int run = 0;
+#pragma unroll 8
+        for (int w = 0; w < kWarpsHere; ++w) {
+            const int c = counters[w * E + e];
+            counters[w * E + e] = run;
+            run += c;
+        }
+        counts[e * gridDim.x + blockIdx.x] = run;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int r = 0; r < steps; ++r) {
+        const int i = first + r * 32 + lane, id = load_id<IdT>(a.ids, i, a.n, E);
+        if (id >= 0) a.row_of[i] += counters[warp * E + id];
+    }
+}
+
+template <typename IdT>
+__global__ void __launch_bounds__(kRouteThreads, 1) route_place_kernel(RouteArgs a, const int* counts) {
+    pdl_prologue();
+    __shared__ int base[kMaxExperts];               // first row of this CTA's entries of an expert
+    __shared__ int filled[kMaxExperts];             // the expert's entries, then the end of its entries (row)
+    __shared__ int ends[kMaxExperts];               // end of the expert's rows
+    __shared__ int warp_total[32];
+    constexpr int kWarpsHere = kRouteThreads / 32;
+    const int E = a.experts, ctas = (int)gridDim.x, rank = (int)blockIdx.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kGroup = 8;                       // experts whose loads are in flight together
+    for (int e0 = warp; e0 < E; e0 += kGroup * kWarpsHere) {
+        int before[kGroup] = {}, total[kGroup] = {};
+#pragma unroll 2
+        for (int c = lane; c < ctas; c += 32) {
+            int v[kGroup];
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) v[g] = e0 + g * kWarpsHere < E ? counts[(e0 + g * kWarpsHere) * ctas + c] : 0;
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) {
+                total[g] += v[g];
+                if (c < rank) before[g] += v[g];
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+            if (e0 + g * kWarpsHere >= E) break;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                before[g] += __shfl_xor_sync(0xffffffffu, before[g], o);
+                total[g] += __shfl_xor_sync(0xffffffffu, total[g], o);
+            }
+            if (lane == 0) { base[e0 + g * kWarpsHere] = before[g]; filled[e0 + g * kWarpsHere] = total[g]; }
+        }
+    }
+    __syncthreads();
+    const int total = tid < E ? filled[tid] : 0, padded = (total + a.block - 1) / a.block * a.block;
+    int end = padded;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += v;
+    }
+    if (lane == 31) warp_total[warp] = end;
+    __syncthreads();
+    if (warp == 0) {
+        int v = warp_total[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        warp_total[lane] = v;
+    }
+    __syncthreads();
+    if (warp > 0) end += warp_total[warp - 1];
+    if (tid < E) {
+        base[tid] += end - padded;
+        filled[tid] = end - padded + total;
+        ends[tid] = end;
+        if (rank == 0) {
+            a.offsets[tid + 1] = min(end, a.rows);
+            if (tid == 0) a.offsets[0] = 0;
+        }
+    }
+    __syncthreads();
+    const int first = (rank * kWarpsHere + warp) * a.per_warp;
+    const int steps = first < a.n ? (min(a.per_warp, a.n - first) + 31) / 32 : 0;
+#pragma unroll 4
+    for (int r = 0; r < steps; ++r) {
+        const int i = first + r * 32 + lane, id = load_id<IdT>(a.ids, i, a.n, E);
+        if (i >= a.n) continue;
+        int row = -1;
+        if (id >= 0) {
+            row = base[id] + a.row_of[i];
+            if (row < a.rows) a.entry_of[row] = i; else row = -1;
+        }
+        a.row_of[i] = row;
+    }
+    // rows without an entry, as above
+    for (int e = rank * kWarpsHere + warp; e < E; e += ctas * kWarpsHere)
+        for (int r = filled[e] + lane; r < min(ends[e], a.rows); r += 32) a.entry_of[r] = -1;
+    for (int r = ends[E - 1] + rank * kRouteThreads + tid; r < a.rows; r += ctas * kRouteThreads) a.entry_of[r] = -1;
 }
 
 // ---------------------------------------------------------------------------
@@ -647,8 +748,8 @@ __global__ void __launch_bounds__(kThreads) combine_bwd_kernel(MoveArgs a) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Threads of a CTA: few entries and experts are sorted sooner by few warps, which meet at every barrier (graph
-// replay: 16 entries over 8 experts 2.8 us, with 1024 threads 3.9; 512 over 64 3.7 and 4.0; but 256 over 256 8.2 and
-// 6.4, 1024 over 32 4.7 and 4.6).
+// replay: 16 entries over 8 experts 2.6 us, with 1024 threads 3.3; 128 over 128 3.2 and 3.4; but 512 over 128 3.85
+// and 3.5, 256 over 256 4.3 and 3.9).
 int route_threads(int64_t n, int64_t experts) {
     return n <= kRouteFewEntries && experts <= kRouteFewExperts ? kRouteFewThreads : kRouteThreads;
 }
@@ -659,13 +760,11 @@ int route_ctas(int64_t n) {
     while (ctas < kRouteMaxCtas && n > (int64_t)ctas * 2 * kRouteThreads) ctas *= 2;
     return ctas;
 }
-int64_t route_per_warp(int64_t n, int ctas, int threads) { return ceil_div(ceil_div(n, ctas * (threads / 32)), 32) * 32; }
-bool route_in_regs(int64_t per_warp) { return per_warp <= 32 * kRouteRegSteps; }
+int64_t route_per_warp(int64_t n, int64_t ctas, int threads) { return ceil_div(ceil_div(n, ctas * (threads / 32)), 32) * 32; }
 size_t route_smem(int64_t n, int64_t experts) {
-    const int ctas = route_ctas(n), threads = route_threads(n, experts), warps = threads / 32;
-    const int64_t per_warp = route_per_warp(n, ctas, threads);
-    const size_t tables = ((size_t)(warps + 5) * experts + (experts & 1)) * sizeof(int);
-    return tables + (route_in_regs(per_warp) ? (size_t)per_warp * warps * sizeof(int2) : 0);
+    if (n > kRouteClusterEntries) return (size_t)(kRouteThreads / 32) * experts * sizeof(int);
+    const int threads = route_threads(n, experts), warps = threads / 32;
+    return ((size_t)(warps + 5) * experts + (experts & 1)) * sizeof(int) + (size_t)route_per_warp(n, route_ctas(n), threads) * warps * sizeof(int2);
 }
 constexpr int kRouteMaxSmem = (kRouteThreads / 32 + 5) * kMaxExperts * (int)sizeof(int) + kRouteThreads * kRouteRegSteps * (int)sizeof(int2);
 static_assert(kRouteMaxSmem + 64 * (int)sizeof(int) <= 227 * 1024, "shared memory of the route kernel");
@@ -700,22 +799,28 @@ int launch_route(const Record& r, cudaStream_t stream, void** p, char* err) {
     a.experts = (int)r.dims[2];
     a.block = (int)r.dims[3];
     a.rows = (int)r.dims[4];
-    const int ctas = (int)r.geom.cluster[0], threads = (int)r.geom.block[0];
+    const bool wide = n > kRouteClusterEntries;
+    const int ctas = (int)r.geom.grid[0], threads = (int)r.geom.block[0];
     a.per_warp = (int)route_per_warp(n, ctas, threads);
-    const int form = threads == kRouteFewThreads ? 0 : route_in_regs(a.per_warp) ? 1 : 2;
-    auto kernel = form == 0 ? route_kernel<IdT, kRouteFewThreads, true>
-                : form == 1 ? route_kernel<IdT, kRouteThreads, true> : route_kernel<IdT, kRouteThreads, false>;
+    const int form = threads == kRouteFewThreads ? 0 : 1;
+    auto kernel = form == 0 ? route_kernel<IdT, kRouteFewThreads> : route_kernel<IdT, kRouteThreads>;
     const size_t smem = route_smem(n, a.experts);
     static std::atomic<uint64_t> attr_set[3];       // bit per device, for the kernels of this id type
+    std::atomic<uint64_t>& done = attr_set[wide ? 2 : form];
     cudaError_t e = cudaSuccess;
     int dev = 0;
     cudaGetDevice(&dev);
-    if (!(attr_set[form].load(std::memory_order_relaxed) & (1ull << (dev & 63)))) {
+    if (!(done.load(std::memory_order_relaxed) & (1ull << (dev & 63)))) {
         // The limit belongs to the kernel, not to a launch: one for all sizes, since another thread may launch another size.
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteMaxSmem);
-        if (e == cudaSuccess) attr_set[form].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+        e = wide ? cudaFuncSetAttribute(route_rank_kernel<IdT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteMaxSmem)
+                 : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteMaxSmem);
+        if (e == cudaSuccess) done.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
     }
-    if (e == cudaSuccess) {
+    if (e == cudaSuccess && wide) {
+        int* counts = (int*)p[4];
+        e = launch_with_pdl(route_rank_kernel<IdT>, dim3(ctas), dim3(threads), smem, stream, a, counts);
+        if (e == cudaSuccess) e = launch_with_pdl(route_place_kernel<IdT>, dim3(ctas), dim3(threads), 0, stream, a, (const int*)counts);
+    } else if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(ctas);
         cfg.blockDim = dim3(threads);
@@ -797,9 +902,15 @@ int plan_moe(Record& r, char* err) {
         if (E > kMaxExperts) { set_err(err, "E=%lld exceeds %d", (long long)E, kMaxExperts); return PB200_ERR_BAD_SHAPE; }
         if (block > kMaxBlock) { set_err(err, "block=%lld exceeds %d", (long long)block, kMaxBlock); return PB200_ERR_BAD_SHAPE; }
         if (rows % block != 0) { set_err(err, "rows=%lld must be divisible by block=%lld", (long long)rows, (long long)block); return PB200_ERR_BAD_SHAPE; }
-        g.cluster[0] = g.grid[0] = (uint32_t)route_ctas(T * k);
-        g.block[0] = (uint32_t)route_threads(T * k, E);
-        g.smem_bytes = (uint32_t)route_smem(T * k, E);
+        const int64_t n = T * k;
+        if (n > kRouteClusterEntries) {
+            g.grid[0] = (uint32_t)ceil_div(n, route_per_warp(n, sm_count(), kRouteThreads) * (kRouteThreads / 32));
+            g.scratch_bytes = (uint64_t)E * g.grid[0] * sizeof(int);
+        } else {
+            g.cluster[0] = g.grid[0] = (uint32_t)route_ctas(n);
+        }
+        g.block[0] = (uint32_t)route_threads(n, E);
+        g.smem_bytes = (uint32_t)route_smem(n, E);
         g.n_inputs = 1;
         g.n_outputs = 3;
         return PB200_OK;

@@ -39,9 +39,10 @@ def _check_route(ids, E, block, rows=None, ids_dtype=None):
 
 @pytest.mark.parametrize("T,k,E,block", [
     (1, 1, 1, 1), (1, 8, 256, 128), (7, 2, 3, 1), (33, 4, 16, 8), (256, 8, 64, 128), (1000, 3, 10, 16),
-    (2049, 1, 1024, 128), (4096, 8, 128, 1), (5000, 32, 32, 100), (8192, 8, 256, 128),     # 1 to 8 CTAs
-    (40000, 8, 60, 128), (9000, 32, 1024, 1),                                              # ranks kept in memory
-    (512, 1, 128, 1), (64, 8, 127, 128), (513, 1, 128, 4), (64, 8, 129, 1), (16, 32, 33, 1024),    # few warps, and just not
+    (2049, 1, 1024, 128), (4096, 8, 128, 1), (8192, 4, 1024, 8), (16000, 2, 61, 128),      # 1 to 8 CTAs
+    (32769, 1, 1, 1), (5000, 32, 32, 100), (8192, 8, 256, 128), (40000, 8, 60, 128), (9000, 32, 1024, 1),      # two launches
+    (512, 1, 128, 1), (64, 8, 127, 128), (513, 1, 128, 4), (64, 8, 129, 1), (16, 32, 33, 1024),
+    (256, 1, 128, 1), (257, 1, 128, 1), (32, 8, 128, 128), (32, 8, 129, 128),              # few warps, and just not
 ])
 @pytest.mark.parametrize("dropped", [0.0, 0.4])
 def test_route_matches_stable_sort(T, k, E, block, dropped):

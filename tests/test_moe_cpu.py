@@ -43,7 +43,9 @@ def test_specs_and_geometry():
     assert route.in_specs[0].dtype is s64 and [s.shape for s in route.out_specs] == [(64, 4), (route.meta["rows"],), (17,)]
     assert route.grid == (1, 1, 1) and route.block == (256, 1, 1)
     assert moe.build_moe_route(64, 4, 256).block == moe.build_moe_route(1024, 4, 16).block == (1024, 1, 1)
-    assert moe.build_moe_route(8192, 8, 64).cluster == (8, 1, 1)
+    assert moe.build_moe_route(8192, 4, 64).cluster == (8, 1, 1) and moe.build_moe_route(8192, 4, 64).scratch_bytes == 0
+    wide = moe.build_moe_route(32769, 1, 64)                   # more than a cluster takes: the counts go through memory
+    assert wide.cluster == (1, 1, 1) and wide.grid[0] > 8 and wide.scratch_bytes == 64 * wide.grid[0] * 4
     d = moe.build_moe_dispatch_fp8(64, 4, 256, 272)
     assert d.out_specs[0].dtype is e4m3 and d.out_specs[1].shape == (256, 3)
     q = build_fp8_quantize(300, 272, block_rows=128, in_dtype=f32)
