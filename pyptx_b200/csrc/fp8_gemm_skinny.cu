@@ -199,7 +199,7 @@ int launch_fp8_skinny(const Record& r, int64_t m, int64_t n, int64_t k, cudaStre
     a.out = ptrs[4];
     a.m = (int)m; a.n = (int)n; a.k = (int)k;
     a.blocks = (int)((k + kBlock - 1) / kBlock);
-    const int warps = fp8_skinny_warps(n, k), token_tiles = m <= 8 ? 1 : 2;
+    const int warps = fp8_skinny_warps(n, k), token_tiles = m <= 8 ? 1 : m <= 16 ? 2 : 4;
     const size_t smem = (size_t)warps * kRows * 8 * token_tiles * sizeof(float);
     const dim3 grid((unsigned)fp8_skinny_grid(n)), block(32 * warps);
     const bool b16 = (r.flags & PB200_F_OUT_BF16) != 0;
@@ -207,9 +207,12 @@ int launch_fp8_skinny(const Record& r, int64_t m, int64_t n, int64_t k, cudaStre
     if (token_tiles == 1)
         e = b16 ? launch_with_pdl(fp8_skinny_kernel<1, 3, __nv_bfloat16>, grid, block, smem, stream, a)
                 : launch_with_pdl(fp8_skinny_kernel<1, 3, float>, grid, block, smem, stream, a);
-    else
+    else if (token_tiles == 2)
         e = b16 ? launch_with_pdl(fp8_skinny_kernel<2, 2, __nv_bfloat16>, grid, block, smem, stream, a)
                 : launch_with_pdl(fp8_skinny_kernel<2, 2, float>, grid, block, smem, stream, a);
+    else                          // one block a warp (make_plan): no depth, which would not fit the registers
+        e = b16 ? launch_with_pdl(fp8_skinny_kernel<4, 1, __nv_bfloat16>, grid, block, smem, stream, a)
+                : launch_with_pdl(fp8_skinny_kernel<4, 1, float>, grid, block, smem, stream, a);
     if (e != cudaSuccess) { set_err(err, "fp8 gemm launch failed (few rows): %s", cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
     return PB200_OK;
 }

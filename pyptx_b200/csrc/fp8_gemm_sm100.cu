@@ -587,7 +587,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Tile shape and split of K.
 //   8 rows at most, dense: the streaming kernel of fp8_gemm_skinny.cu (1 x 4096 x 4096 from HBM: 4.9 us against
 //   7.0 on 32 x 128 tiles), with 9 to 16 rows up to 16 Mi weights, since its arithmetic doubles (16 x 4096 x 4096:
-//   6.4 against 7.4 us, but 16 x 8192 x 8192: 19.5 against 15).
+//   6.4 against 7.4 us, but 16 x 8192 x 8192: 19.5 against 15), and with 17 to 32 rows up to 4 Mi weights where a warp
+//   has one block of K (32 x 2048 x 2048: 4.5 against 5.8 us, 32 x 1024 x 1024: 3.6 against 4.4; but 32 x 4096 x 2048
+//   6.2 against 6.1 and 32 x 1024 x 4096, two blocks a warp, 6.7 against 5.7).
 //   few rows: 32 x 128 tiles; dense up to 32 rows (32 x 4096 x 4096: 7.5 us, on 128 x 128 tiles 7.7), grouped up to 24
 //   for each expert on average, since loads are uneven (32 experts, 4096 x 2048: 24 rows 48.6 us, on 128 x 128 tiles
 //   52.3; 28 rows 54.5 and 52.8).
@@ -615,7 +617,8 @@ Plan make_plan(const Record& r) {
     p.m = d[0]; p.n = d[1]; p.k = d[2];
     p.split = 1;
     const int64_t sms = sm_count(), mean_rows = grouped ? ceil_div(p.m, p.experts) : p.m;
-    if (!grouped && (p.m <= 8 || (p.m <= 16 && p.n * p.k <= (1 << 24)))) {
+    if (!grouped && (p.m <= 8 || (p.m <= 16 && p.n * p.k <= (1 << 24)) ||
+                     (p.m <= 32 && p.n * p.k <= (1 << 22) && ceil_div(p.k, BK) <= fp8_skinny_warps(p.n, p.k)))) {
         p.skinny = true;
         p.tiles = fp8_skinny_grid(p.n);
         return p;

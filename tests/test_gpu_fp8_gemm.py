@@ -88,6 +88,7 @@ def test_every_scale_block_counts_once():
 
 @pytest.mark.parametrize("M,N,K", [
     (1, 8, 16), (1, 4096, 4096), (2, 136, 128), (3, 520, 2064), (8, 2056, 8208), (9, 1016, 528), (16, 1024, 4096), (17, 72, 5120), (24, 4104, 2048), (12, 8200, 2064), (31, 264, 144), (32, 256, 256),
+    (17, 1024, 1024), (32, 2048, 2048), (25, 1000, 528), (32, 8, 16), (28, 4096, 1024), (31, 520, 2176),
     (33, 256, 384), (64, 2056, 1040), (127, 128, 512), (128, 384, 640), (129, 248, 272), (333, 2056, 1040),
     (512, 512, 16), (1000, 1000, 1008), (2048, 2048, 256), (1030, 4104, 528), (4000, 1544, 400), (8192, 264, 128),
 ])
@@ -98,9 +99,9 @@ def test_dense(M, N, K, kind):
     _check(d, a, sa, b, sb, kind)
 
 
-@pytest.mark.parametrize("M", [10, 16, 20, 40])            # streaming, 32-row and 128-row forms
-def test_special_scales_and_values_stay_in_their_rows(M):
-    N, K = 256, 512
+@pytest.mark.parametrize("M,N,K", [(10, 256, 512), (16, 256, 512), (20, 256, 512), (28, 520, 4224), (40, 256, 512)])
+def test_special_scales_and_values_stay_in_their_rows(M, N, K):
+    """Streaming, 32-row and 128-row forms."""
     a, sa, b, sb = _operands(M, N, K, 5)
     clean = build_fp8_gemm(M, N, K)(a.cuda(), sa.cuda(), b.cuda(), sb.cuda())
     a2, sa2 = a.float(), sa.clone()
@@ -130,8 +131,7 @@ def test_tiles_in_quick_succession(M, N, K, kind):
 
 
 def test_special_weights_stay_in_their_columns():
-    for M in (3, 20, 200):
-        N, K = 384, 256
+    for M, N, K in ((3, 384, 256), (20, 384, 256), (20, 384, 2304), (200, 384, 256)):
         a, sa, b, sb = _operands(M, N, K, 6)
         clean = build_fp8_gemm(M, N, K)(a.cuda(), sa.cuda(), b.cuda(), sb.cuda())
         b2, sb2 = b.float(), sb.clone()
