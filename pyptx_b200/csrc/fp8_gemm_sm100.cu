@@ -596,9 +596,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   dense: 128 x 128 tiles while they fit the SMs at once (512 x 4096 x 4096: 11.6 us, as pairs 16.2), else
 //   256 x 256 tiles of CTA pairs (768 x 4096 x 4096: 17.0 us, as 128 x 128 ones one after the other 21.3),
 //   unless a pair's tile would be half empty (40000 x 128 x 4096: 42 us, as pairs 50).  Where 128-column tiles
-//   leave SMs idle the K blocks of a tile are shared by a cluster of up to 8 CTAs (at least eight blocks each:
-//   the cluster's two barriers take about 1.6 us), which add their partial tiles through distributed shared
-//   memory in a fixed order.
+//   leave SMs idle the K blocks of a tile, if they are 20 or more, are shared by a cluster of up to 8 CTAs (at
+//   least eight blocks each: the cluster's two barriers take about 1.6 us), which add their partial tiles through
+//   distributed shared memory in a fixed order (256 rows and 2048 x 2048: 6.9 us, shared by two 7.5; 64 rows and
+//   2048 x 3584: 9.1 and 7.8; 64 rows and 4096 x 4096: by two 8.9, by four 8.4).
 //   grouped: the tiles are known on the device only, so the rows an expert has on average decide: pairs from
 //   128 (32 experts, 4096 x 2048: 96 rows 60 us on 128 x 128 tiles, 71 as pairs; 128 rows 74.7 and 72.2; 200 rows
 //   92 and 75).
@@ -633,7 +634,7 @@ Plan make_plan(const Record& r) {
         // A cluster lives in one GPC, so only so many run at once: 15 of 8 CTAs and 33 of 4 were seen to (a
         // 16th doubles 32 x 2048 x 8192 from 8.0 to 13.6 us), and GPUs differ in which SMs they have.
         auto fits = [&](int64_t split) { return p.tiles * split <= (split == 8 ? sms * 3 / 4 : split == 4 ? sms * 7 / 8 : sms); };
-        while (p.split < kMaxSplit && fits(p.split * 2) && blocks >= 16 * p.split) p.split *= 2;
+        while (p.split < kMaxSplit && fits(p.split * 2) && blocks >= (p.split == 1 ? 20 : 16 * p.split)) p.split *= 2;
     }
     return p;
 }

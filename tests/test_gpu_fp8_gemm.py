@@ -89,6 +89,7 @@ def test_every_scale_block_counts_once():
 @pytest.mark.parametrize("M,N,K", [
     (1, 8, 16), (1, 4096, 4096), (2, 136, 128), (3, 520, 2064), (8, 2056, 8208), (9, 1016, 528), (16, 1024, 4096), (17, 72, 5120), (24, 4104, 2048), (12, 8200, 2064), (31, 264, 144), (32, 256, 256),
     (17, 1024, 1024), (32, 2048, 2048), (25, 1000, 528), (32, 8, 16), (28, 4096, 1024), (31, 520, 2176),
+    (300, 1000, 2576), (40, 1024, 4096), (33, 264, 8992), (20, 200, 8208), (130, 2056, 2640),      # K shared by 2 to 8 CTAs
     (33, 256, 384), (64, 2056, 1040), (127, 128, 512), (128, 384, 640), (129, 248, 272), (333, 2056, 1040),
     (512, 512, 16), (1000, 1000, 1008), (2048, 2048, 256), (1030, 4104, 528), (4000, 1544, 400), (8192, 264, 128),
 ])
