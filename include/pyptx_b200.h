@@ -191,6 +191,8 @@ extern "C" {
  *   a_scale[m,b] * b_scale[n/128,b] * sum_{k in b} A[m,k] B_T[n,k]
  * (the 8-bit counterpart of PB200_K_GEMM_1SM and PB200_K_GROUPED_GEMM_VARLEN; the reference has no
  * 8-bit GEMM).  K % 16 == 0, N % 8 == 0, M free.   flags: PB200_F_OUT_BF16
+ * a_scale * b_scale is formed in f32: a product below 2^-126 is rounded to a multiple of 2^-149 (an error of at
+ * most 2^-125 for each block), one of 2^128 and more is infinite (inf, or NaN over a block of zeros).
  *   PB200_K_FP8_GEMM          dims = {M, N, K}
  *       buffers: A[M,K] e4m3, a_scale[M,ceil(K/128)] f32, B_T[N,K] e4m3,
  *                b_scale[ceil(N/128),ceil(K/128)] f32 -> D[M,N] f32 (or bf16)

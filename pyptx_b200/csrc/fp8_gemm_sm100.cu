@@ -9,6 +9,10 @@
 // runs in registers: the epilogue warps fetch each block's accumulator from TMEM, multiply it by the
 // row's scale times the weight block's and add it to the tile's f32 sums.  128 rows are the 128 TMEM
 // lanes, so a thread has one row: one scale for a block of K, and its columns lie in one weight block.
+// The two scales are multiplied first, in f32, one product a block: products below 2^-126 lose bits (2^-125 of a block's
+// result at most) and those of 2^128 are infinite.  Looking out for them costs every call more than it gives: a vote a
+// block and a branch 239 us at 8192 x 8192 x 4096 where 215 were measured without, a look by the warp that copies the scales
+// 229, sums kept at 2^24 times their value 217 (and those overflow sooner).
 //
 // What bounds it at large sizes: a CTA's 128 x 256 x 128 block takes 512 clocks of MMA, 512 of operands
 // from L2 (64 bytes a clock), and the drain of its accumulators 286 clocks of each SM sub-partition's

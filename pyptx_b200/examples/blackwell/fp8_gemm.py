@@ -3,6 +3,12 @@
 Operands are e4m3 with f32 scales: activations one for each row and 128 columns, weights one for each
 128 x 128 block.  The reference has no 8-bit GEMM; the dense product stands beside ``build_gemm`` and
 the grouped one beside ``build_grouped_gemm_varlen``.
+
+The product of a row's and a weight block's scale is formed in f32 before it meets the block's sum (which is 0
+or between 2^-18 and 2^24.6).  Scales whose products lie in 2^-126 .. 2^127 are what these products are for.  A
+smaller one is rounded to f32's subnormal step, which is an error of at most 2^-125 for each block of K; one of
+2^128 and more is infinite, and the results of its row and column block infinite or NaN (a block of zeros
+included).
 """
 from __future__ import annotations
 
@@ -53,7 +59,8 @@ def build_fp8_gemm(M: int, N: int, K: int, *, out_dtype: PtxType = f32, arch: st
 
     The operands are what ``build_fp8_quantize`` returns (``block_rows=1`` for ``A``, 128 for the weight
     ``B_T``, which is K-major as in ``build_gemm``).  ``M`` is free, from single tokens on; ``N`` divides by 8
-    and ``K`` by 16.  Products within a block and the scaled sum over blocks are accumulated in f32.  The
+    and ``K`` by 16.  Products within a block and the scaled sum over blocks are accumulated in f32 (the range of
+    the scales' products: see the module).  The
     gradient for the inputs is the same product: ``dX = k'(dY, W^T)``, the weight's bytes and its grid of
     scales transposed.
     """
