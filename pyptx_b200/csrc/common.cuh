@@ -21,6 +21,7 @@ struct Record {
     double   fparams[4] = {0, 0, 0, 0};
     int      n_fparams = 0;
     uint64_t flags     = 0;
+    int      steps     = 0;       // the movement kernels' choice at create time (moe_sm100.cu)
     pb200_geometry geom{};
 };
 
@@ -66,6 +67,7 @@ int launch_fp8_gemm(const Record& r, cudaStream_t stream, void** ptrs, char* err
 // The dense product's form for few rows (fp8_gemm_skinny.cu).
 int fp8_skinny_warps(int64_t n, int64_t k);
 int64_t fp8_skinny_grid(int64_t n);
+size_t fp8_skinny_smem(int64_t m, int64_t n, int64_t k);
 int launch_fp8_skinny(const Record& r, int64_t m, int64_t n, int64_t k, cudaStream_t stream, void** ptrs, char* err);
 
 // Device-side status word (defined in abi.cu's translation unit of the same

@@ -189,6 +189,10 @@ int fp8_skinny_warps(int64_t n, int64_t k) {
     return (int)(blocks < warps ? blocks : warps);
 }
 int64_t fp8_skinny_grid(int64_t n) { return (n + kRows - 1) / kRows; }
+static int token_tiles_of(int64_t m) { return m <= 8 ? 1 : m <= 16 ? 2 : 4; }
+size_t fp8_skinny_smem(int64_t m, int64_t n, int64_t k) {
+    return (size_t)fp8_skinny_warps(n, k) * kRows * 8 * token_tiles_of(m) * sizeof(float);
+}
 
 int launch_fp8_skinny(const Record& r, int64_t m, int64_t n, int64_t k, cudaStream_t stream, void** ptrs, char* err) {
     SkinnyArgs a;
@@ -199,9 +203,9 @@ int launch_fp8_skinny(const Record& r, int64_t m, int64_t n, int64_t k, cudaStre
     a.out = ptrs[4];
     a.m = (int)m; a.n = (int)n; a.k = (int)k;
     a.blocks = (int)((k + kBlock - 1) / kBlock);
-    const int warps = fp8_skinny_warps(n, k), token_tiles = m <= 8 ? 1 : m <= 16 ? 2 : 4;
-    const size_t smem = (size_t)warps * kRows * 8 * token_tiles * sizeof(float);
-    const dim3 grid((unsigned)fp8_skinny_grid(n)), block(32 * warps);
+    const int token_tiles = token_tiles_of(m);
+    const size_t smem = fp8_skinny_smem(m, n, k);
+    const dim3 grid((unsigned)fp8_skinny_grid(n)), block(32 * fp8_skinny_warps(n, k));
     const bool b16 = (r.flags & PB200_F_OUT_BF16) != 0;
     cudaError_t e;
     if (token_tiles == 1)

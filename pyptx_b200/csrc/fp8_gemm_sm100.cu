@@ -750,6 +750,7 @@ int plan_fp8_gemm(Record& r, char* err) {
     if (p.skinny) {
         g.grid[0] = (uint32_t)p.tiles;
         g.block[0] = (uint32_t)(32 * fp8_skinny_warps(p.n, p.k));
+        g.smem_bytes = (uint32_t)fp8_skinny_smem(p.m, p.n, p.k);
         return PB200_OK;
     }
     g.grid[0] = (uint32_t)grid_of(p);

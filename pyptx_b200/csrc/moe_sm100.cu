@@ -780,9 +780,49 @@ int pick_steps(int64_t rows, int64_t width, int64_t step, int most) {
     return u;
 }
 
+// How a movement or row-quantising kernel walks its rows of `width` (16-byte vectors, or columns where it quantises):
+// `steps` of a warp make a segment, `zero_units` clear 32 rows' segments each, `grid` CTAs in all.
+struct Walk {
+    int64_t width, segs, zero_units, grid;
+};
+Walk walk_of(const Record& r, int steps) {
+    const int64_t T = r.dims[0], H = r.dims[3];
+    const int64_t vecs = H * ((r.flags & PB200_F_OUT_BF16) ? 2 : 4) / 16;
+    Walk w{};
+    switch (r.kernel_id) {
+    case PB200_K_FP8_QUANTIZE:
+    case PB200_K_MOE_DISPATCH_FP8:
+        w.width = r.kernel_id == PB200_K_FP8_QUANTIZE ? r.dims[1] : H;
+        w.segs = ceil_div(w.width, 256 * steps);
+        break;
+    case PB200_K_MOE_COMBINE_BWD:                   // a CTA a token; its segments are those of the rows to clear
+        w.width = vecs;
+        w.segs = ceil_div(vecs, 128);
+        break;
+    default:
+        w.width = vecs;
+        w.segs = ceil_div(vecs, 32 * steps);
+    }
+    const bool clears = r.kernel_id == PB200_K_MOE_DISPATCH || r.kernel_id == PB200_K_MOE_DISPATCH_FP8 || r.kernel_id == PB200_K_MOE_COMBINE_BWD;
+    w.zero_units = clears ? ceil_div(r.dims[2], 32) * w.segs : 0;
+    w.grid = r.kernel_id == PB200_K_MOE_COMBINE_BWD ? ceil_div(w.zero_units, kWarps) + T : ceil_div(w.zero_units + T * w.segs, kWarps);
+    return w;
+}
+// The steps of a handle, chosen when it is made.
+int steps_of(const Record& r) {
+    const int64_t width = walk_of(r, 1).width;
+    switch (r.kernel_id) {
+    case PB200_K_FP8_QUANTIZE:
+    case PB200_K_MOE_DISPATCH_FP8: return pick_steps(r.dims[0], width, 256, 4);
+    case PB200_K_MOE_DISPATCH:     return pick_steps(r.dims[0], width, 32, 4);
+    case PB200_K_MOE_COMBINE_BWD:  return 4;
+    default:                       return pick_steps(r.dims[0], width, 32, 2);
+    }
+}
+
 template <typename... KArgs, typename... Args>
-int enqueue(const char* what, void (*kernel)(KArgs...), int64_t grid, int threads, cudaStream_t stream, char* err, Args... args) {
-    cudaError_t e = launch_with_pdl(kernel, dim3((unsigned)grid), dim3(threads), 0, stream, args...);
+int enqueue(const char* what, void (*kernel)(KArgs...), const Record& r, cudaStream_t stream, char* err, Args... args) {
+    cudaError_t e = launch_with_pdl(kernel, dim3(r.geom.grid[0]), dim3(r.geom.block[0]), 0, stream, args...);
     if (e != cudaSuccess) { set_err(err, "%s launch failed: %s", what, cudaGetErrorString(e)); return PB200_ERR_LAUNCH; }
     return PB200_OK;
 }
@@ -848,25 +888,21 @@ MoveArgs move_args(const Record& r, int64_t width, int elt_bytes) {
     a.width = (int)width;
     a.vecs = (int)(width * elt_bytes / 16);
     a.scale_cols = (int)ceil_div(width, kScaleBlock);
+    const Walk w = walk_of(r, r.steps);
+    a.segs = (int)w.segs;
+    a.zero_units = w.zero_units;
     return a;
 }
 
 template <typename T, bool ROUTED>
-int launch_quantize_rows(MoveArgs a, cudaStream_t stream, char* err) {
-    const int u = pick_steps(a.tokens, a.width, 256, 4);
-    a.segs = (int)ceil_div(a.width, 256 * u);
-    a.zero_units = ROUTED ? ceil_div(a.rows, 32) * a.segs : 0;
-    const int64_t grid = ceil_div(a.zero_units + a.tokens * a.segs, kWarps);
-    auto kernel = u == 4 ? quantize_rows_kernel<T, 4, ROUTED> : u == 2 ? quantize_rows_kernel<T, 2, ROUTED> : quantize_rows_kernel<T, 1, ROUTED>;
-    return enqueue("fp8 quantisation", kernel, grid, kThreads, stream, err, a);
+int launch_quantize_rows(const Record& r, MoveArgs a, cudaStream_t stream, char* err) {
+    auto kernel = r.steps == 4 ? quantize_rows_kernel<T, 4, ROUTED> : r.steps == 2 ? quantize_rows_kernel<T, 2, ROUTED> : quantize_rows_kernel<T, 1, ROUTED>;
+    return enqueue("fp8 quantisation", kernel, r, stream, err, a);
 }
 
 template <typename T, bool WEIGHTED>
-int launch_combine(MoveArgs a, cudaStream_t stream, char* err) {
-    const int u = pick_steps(a.tokens, a.vecs, 32, 2);
-    a.segs = (int)ceil_div(a.vecs, 32 * u);
-    return enqueue("moe_combine", u == 1 ? combine_kernel<T, 1, WEIGHTED> : combine_kernel<T, 2, WEIGHTED>,
-                   ceil_div(a.tokens * a.segs, kWarps), kThreads, stream, err, a);
+int launch_combine(const Record& r, MoveArgs a, cudaStream_t stream, char* err) {
+    return enqueue("moe_combine", r.steps == 1 ? combine_kernel<T, 1, WEIGHTED> : combine_kernel<T, 2, WEIGHTED>, r, stream, err, a);
 }
 
 }  // namespace
@@ -888,8 +924,13 @@ int plan_moe(Record& r, char* err) {
         if (r.dims[2] != 1 && r.dims[2] != kScaleBlock) return bad("block_rows must be 1 or 128");
         const int64_t grid = r.dims[2] == 1 ? ceil_div(M * ceil_div(K, 256), kWarps) : ceil_div(M, kScaleBlock) * ceil_div(K, kScaleBlock);
         if (grid > 0x7fffffffLL) return bad("matrix is too large for one launch");
-        g.grid[0] = (uint32_t)grid;
-        if (r.dims[2] != 1) g.block[0] = kBlockThreads;
+        if (r.dims[2] == 1) {
+            r.steps = steps_of(r);
+            g.grid[0] = (uint32_t)walk_of(r, r.steps).grid;
+        } else {
+            g.grid[0] = (uint32_t)grid;
+            g.block[0] = kBlockThreads;
+        }
         g.n_inputs = 1;
         g.n_outputs = 2;
         return PB200_OK;
@@ -921,7 +962,8 @@ int plan_moe(Record& r, char* err) {
     if (H % unit != 0) { set_err(err, "H=%lld must be divisible by %d", (long long)H, unit); return PB200_ERR_BAD_SHAPE; }
     // one warp for each 32 vectors at most, and the same again for rows to clear
     if (ceil_div(T + ceil_div(rows, 32), 1) * ceil_div(H, 128) > 0x7fffffffLL) return bad("tensor is too large for one launch");
-    g.grid[0] = (uint32_t)ceil_div(T * ceil_div(H, 128), kWarps);
+    r.steps = steps_of(r);
+    g.grid[0] = (uint32_t)walk_of(r, r.steps).grid;
     switch (r.kernel_id) {
         case PB200_K_MOE_DISPATCH:     g.n_inputs = 3; g.n_outputs = 1; break;
         case PB200_K_MOE_DISPATCH_FP8: g.n_inputs = 3; g.n_outputs = 2; break;
@@ -940,36 +982,29 @@ int launch_moe(const Record& r, cudaStream_t stream, void** p, char* err) {
     case PB200_K_MOE_DISPATCH: {
         MoveArgs a = move_args(r, r.dims[3], b16 ? 2 : 4);
         a.src = p[0]; a.row_of = (const int*)p[1]; a.entry_of = (const int*)p[2]; a.dst = p[3];
-        const int u = pick_steps(a.tokens, a.vecs, 32, 4);
-        a.segs = (int)ceil_div(a.vecs, 32 * u);
-        a.zero_units = ceil_div(a.rows, 32) * a.segs;
-        return enqueue("moe_dispatch", u == 1 ? dispatch_kernel<1> : u == 2 ? dispatch_kernel<2> : dispatch_kernel<4>,
-                       ceil_div(a.zero_units + a.tokens * a.segs, kWarps), kThreads, stream, err, a);
+        return enqueue("moe_dispatch", r.steps == 1 ? dispatch_kernel<1> : r.steps == 2 ? dispatch_kernel<2> : dispatch_kernel<4>, r, stream, err, a);
     }
     case PB200_K_MOE_DISPATCH_FP8: {
         MoveArgs a = move_args(r, r.dims[3], 1);
         a.src = p[0]; a.row_of = (const int*)p[1]; a.entry_of = (const int*)p[2]; a.dst = p[3]; a.dst_scale = (float*)p[4];
-        return in_b16 ? launch_quantize_rows<__nv_bfloat16, true>(a, stream, err) : launch_quantize_rows<float, true>(a, stream, err);
+        return in_b16 ? launch_quantize_rows<__nv_bfloat16, true>(r, a, stream, err) : launch_quantize_rows<float, true>(r, a, stream, err);
     }
     case PB200_K_MOE_DISPATCH_BWD: {
         MoveArgs a = move_args(r, r.dims[3], b16 ? 2 : 4);
         a.row_of = (const int*)p[0]; a.src = p[1]; a.dst = p[2];
-        return b16 ? launch_combine<__nv_bfloat16, false>(a, stream, err) : launch_combine<float, false>(a, stream, err);
+        return b16 ? launch_combine<__nv_bfloat16, false>(r, a, stream, err) : launch_combine<float, false>(r, a, stream, err);
     }
     case PB200_K_MOE_COMBINE: {
         MoveArgs a = move_args(r, r.dims[3], b16 ? 2 : 4);
         a.src = p[0]; a.weights = (const float*)p[1]; a.row_of = (const int*)p[2]; a.dst = p[3];
-        return b16 ? launch_combine<__nv_bfloat16, true>(a, stream, err) : launch_combine<float, true>(a, stream, err);
+        return b16 ? launch_combine<__nv_bfloat16, true>(r, a, stream, err) : launch_combine<float, true>(r, a, stream, err);
     }
     case PB200_K_MOE_COMBINE_BWD: {
         MoveArgs a = move_args(r, r.dims[3], b16 ? 2 : 4);
         a.src = p[0]; a.weights = (const float*)p[1]; a.row_of = (const int*)p[2]; a.entry_of = (const int*)p[3]; a.grad = p[4];
         a.d_rows = p[5]; a.d_weights = (float*)p[6];
-        a.segs = (int)ceil_div(a.vecs, 128);
-        a.zero_units = ceil_div(a.rows, 32) * a.segs;
-        const int64_t grid = ceil_div(a.zero_units, kWarps) + a.tokens;
-        return b16 ? enqueue("moe_combine_bwd", combine_bwd_kernel<__nv_bfloat16, 4>, grid, kThreads, stream, err, a)
-                   : enqueue("moe_combine_bwd", combine_bwd_kernel<float, 4>, grid, kThreads, stream, err, a);
+        return b16 ? enqueue("moe_combine_bwd", combine_bwd_kernel<__nv_bfloat16, 4>, r, stream, err, a)
+                   : enqueue("moe_combine_bwd", combine_bwd_kernel<float, 4>, r, stream, err, a);
     }
     default: break;
     }
@@ -977,17 +1012,16 @@ int launch_moe(const Record& r, cudaStream_t stream, void** p, char* err) {
     const int64_t M = r.dims[0], K = r.dims[1];
     if (r.dims[2] == 1) {
         MoveArgs a{};
-        a.tokens = M; a.width = (int)K; a.scale_cols = (int)ceil_div(K, kScaleBlock);
+        a.tokens = M; a.width = (int)K; a.scale_cols = (int)ceil_div(K, kScaleBlock); a.segs = (int)walk_of(r, r.steps).segs;
         a.src = p[0]; a.dst = p[1]; a.dst_scale = (float*)p[2];
-        return in_b16 ? launch_quantize_rows<__nv_bfloat16, false>(a, stream, err) : launch_quantize_rows<float, false>(a, stream, err);
+        return in_b16 ? launch_quantize_rows<__nv_bfloat16, false>(r, a, stream, err) : launch_quantize_rows<float, false>(r, a, stream, err);
     }
     const int sc = (int)ceil_div(K, kScaleBlock);
-    const int64_t grid = ceil_div(M, kScaleBlock) * sc;
     if (in_b16)
-        return enqueue("fp8 quantisation", quantize_blocks_kernel<__nv_bfloat16>, grid, kBlockThreads, stream, err,
-                       (const __nv_bfloat16*)p[0], (uint8_t*)p[1], (float*)p[2], M, (int)K, sc);
-    return enqueue("fp8 quantisation", quantize_blocks_kernel<float>, grid, kBlockThreads, stream, err, (const float*)p[0],
-                   (uint8_t*)p[1], (float*)p[2], M, (int)K, sc);
+        return enqueue("fp8 quantisation", quantize_blocks_kernel<__nv_bfloat16>, r, stream, err, (const __nv_bfloat16*)p[0],
+                       (uint8_t*)p[1], (float*)p[2], M, (int)K, sc);
+    return enqueue("fp8 quantisation", quantize_blocks_kernel<float>, r, stream, err, (const float*)p[0], (uint8_t*)p[1],
+                   (float*)p[2], M, (int)K, sc);
 }
 
 }  // namespace pb200
