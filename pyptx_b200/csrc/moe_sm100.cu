@@ -30,7 +30,7 @@ constexpr int kMaxTopK = 32;                  // one lane holds one choice's row
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxBlock = 1024;
 constexpr int kScaleBlock = 128;
-constexpr int64_t kMaxExtent = 0x7fff0000;    // rows and columns; 65535 more still fit 32 bits (a grid's step past the last need not)
+constexpr int64_t kMaxExtent = 0x7fff0000;    // rows and columns; 65535 more fit 32 bits (a whole grid's step past the last need not)
 
 __device__ __forceinline__ void pdl_prologue() {
     ptx::pdl_launch_dependents();
@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(THREADS, 1) route_kernel(RouteArgs a) {
     // rows without an entry: each expert's padding, then everything behind the last expert
     for (int e = rank * kWarpsHere + warp; e < E; e += (int)n_ctas * kWarpsHere)
         for (int r = filled[e] + lane; r < min(ends[e], a.rows); r += 32) a.entry_of[r] = -1;
-    for (int64_t r = ends[E - 1] + rank * THREADS + tid; r < a.rows; r += (int)n_ctas * THREADS) a.entry_of[r] = -1;
+    static_assert(kMaxExtent + kRouteMaxCtas * kRouteThreads <= 0x7fffffff, "a cluster's step past the last row fits 32 bits");
+    for (int r = ends[E - 1] + rank * THREADS + tid; r < a.rows; r += (int)n_ctas * THREADS) a.entry_of[r] = -1;
     if (n_ctas > 1) ptx::cluster_wait();            // shared memory must outlive the other CTAs' reads
 }
 
