@@ -15,7 +15,9 @@
 // None for whatever it does not accept, and the caller takes the checking path, which words the errors.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/Context.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -110,6 +112,11 @@ public:
             ptrs[i] = t.data_ptr();
         }
         if (c10::cuda::current_device() != device.index()) return decline();
+        // Allocations that somebody wants to see or have filled go through the dispatcher: a dispatch mode is active, or
+        // torch fills what a kernel may leave unwritten (torch.utils.deterministic.fill_uninitialized_memory).
+        if (c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+            (at::globalContext().deterministicAlgorithms() && at::globalContext().deterministicFillUninitializedMemory()))
+            return decline();
         const uint64_t stream = (uint64_t)(uintptr_t)c10::cuda::getCurrentCUDAStream(device.index()).stream();
         c10::SmallVector<at::Tensor, 4> outs;
         for (size_t i = 0; i < out_shapes_.size(); ++i) {
