@@ -30,3 +30,37 @@ def test_route_with_the_most_rows_that_are_accepted(T):
     assert torch.equal(words[guard:guard + T].cpu(), want[1])
     assert bool((words[:guard] == -7).all()), "words before entry_of were written"
     assert bool((words[guard + T:] == -1).all()), "a row without an entry was left out"
+
+
+def test_threads_whose_sorts_need_different_shared_memory():
+    """Three sorts of the same kernel, each above the 48 KB that a launch gets unasked, and a fourth of the two-launch
+    form: one thread's smaller limit must not reach another's launch."""
+    import threading
+
+    shapes = [(32768, 1, 1024, 184320), (2048, 1, 330, 57032), (16384, 1, 1000, 164384), (40000, 1, 600, 76800)]
+    routes = [moe.build_moe_route(T, k, E, block=1) for T, k, E, _ in shapes]
+    assert [r.smem for r in routes] == [s[3] for s in shapes] and all(r.block == (1024, 1, 1) for r in routes)
+    ids = [torch.randint(0, E, (T, k), dtype=torch.int32, device="cuda") for T, k, E, _ in shapes]
+    torch.cuda.synchronize()
+    errors, done = [], [0] * len(shapes)
+    start = threading.Barrier(len(shapes))
+
+    def work(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(300):
+                    _, entry_of, _ = routes[n](ids[n])
+                torch.cuda.current_stream().synchronize()
+                order = torch.sort(ids[n].flatten(), stable=True).indices
+                assert torch.equal(entry_of.long(), order)
+            done[n] += 1
+        except Exception as exc:  # noqa: BLE001
+            errors.append(exc)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(len(shapes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and done == [1] * len(shapes), errors
