@@ -60,9 +60,15 @@ def build_fp8_gemm(M: int, N: int, K: int, *, out_dtype: PtxType = f32, arch: st
     The operands are what ``build_fp8_quantize`` returns (``block_rows=1`` for ``A``, 128 for the weight
     ``B_T``, which is K-major as in ``build_gemm``).  ``M`` is free, from single tokens on; ``N`` divides by 8
     and ``K`` by 16.  Products within a block and the scaled sum over blocks are accumulated in f32 (the range of
-    the scales' products: see the module).  The
-    gradient for the inputs is the same product: ``dX = k'(dY, W^T)``, the weight's bytes and its grid of
-    scales transposed.
+    the scales' products: see the module).
+
+    The gradient for the inputs is such a product too, of the gradient in 8 bits and the weight's bytes and grid of
+    scales transposed (128 x 128 blocks stay 128 x 128 blocks)::
+
+        dX = build_fp8_gemm(M, K, N)(*build_fp8_quantize(M, N)(dY), B_T.t().contiguous(), b_scale.t().contiguous())
+
+    ``N`` divides by 16 there (else: eight columns of zeros for ``dY`` and eight rows of zeros for ``B_T``).  The 8-bit
+    weight itself has no gradient.
     """
     assert M >= 1, f"M={M} must be positive"
     _check(N, K, out_dtype)
