@@ -68,7 +68,8 @@ static_assert(kSmemTotal <= 227 * 1024, "shared memory");
 constexpr int kMaxSplit = 8;
 // Registers of the 256-column form, whose epilogue threads hold 128 sums: the launch has 384 x 168;
 // the control warpgroup gives up 128 x 112 of them and the two epilogue warpgroups take 256 x 56 (with 16 a
-// thread more for these and as many less for the control warps, the control warps spill).
+// thread more for these and as many less for the control warps, the control warps spill; as it is, ptxas reports 12 bytes of
+// spill stores for bf16 results and none for f32 ones).
 constexpr int kControlRegs = 56, kEpilogueRegs = 224;
 static_assert(128 * kControlRegs + 256 * kEpilogueRegs <= kLaunchThreads * 168, "register split");     // checked at the first launch too
 
@@ -604,7 +605,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   least eight blocks each: the cluster's two barriers take about 1.6 us), which add their partial tiles through
 //   distributed shared memory in a fixed order (256 rows and 2048 x 2048: 6.9 us, shared by two 7.5; 64 rows and
 //   2048 x 3584: 9.1 and 7.8; 64 rows and 4096 x 4096: by two 8.9, by four 8.4).
-//   grouped: the tiles are known on the device only, so the rows an expert has on average decide: pairs from
+//   grouped: the tiles are known on the device only, so the rows an expert can have on average decide (the capacity:
+//   the figures have buffers that are full; 64 experts of 2 rows in 8192 rows take 63 us, in 128 rows 45): pairs from
 //   128 (32 experts, 4096 x 2048: 96 rows 60 us on 128 x 128 tiles, 71 as pairs; 128 rows 74.7 and 72.2; 200 rows
 //   92 and 75).
 struct Plan {

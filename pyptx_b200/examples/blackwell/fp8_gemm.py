@@ -90,7 +90,9 @@ def build_fp8_grouped_gemm_varlen(G: int, M_total: int, N: int, K: int, *, out_d
     Expert ``e`` owns rows ``[offsets[e], offsets[e+1])`` of ``A`` and ``C`` and its own ``N`` rows of ``B_T``.
     Offsets live on the device, are non-decreasing within ``[0, M_total]`` and, unlike the bf16 kernel's, need
     no alignment, so ``build_moe_route(..., block=1)`` wastes no rows.  Rows outside
-    ``[offsets[0], offsets[G])`` are left unwritten.  ``M_total`` is the static capacity.
+    ``[offsets[0], offsets[G])`` are left unwritten.  ``M_total`` is the static capacity; tiles are chosen by
+    ``M_total / G``, so a buffer sized close to the rows that come is quicker (64 experts of 2 rows, 2048 x 2048: 45 us
+    in 128 rows, 63 in 8192).
     """
     assert 1 <= G <= MAX_EXPERTS, f"G={G} must be in [1, {MAX_EXPERTS}]"
     assert M_total >= 1, f"M_total={M_total} must be positive"
